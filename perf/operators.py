@@ -219,7 +219,7 @@ def prepare_tree(case, seed, s, normal, whole):
           "slots": whole(np.arange(n)), "mask": whole(mask.view(np.int64), torch.int64) if case["mask"] == "tree" else None}
     if own:
         s["pool"] = make_pool(s, [s["k"], s["v"]], s["k"].shape[1] * s["k"].element_size())
-        s["work_bytes"] = context().tree_attn_workspace(rows=rows, n_seqs=n, n_q_heads=hq, n_kv_heads=hkv, head_dim=hd)
+        s["work_bytes"] = context().tree_attn_workspace(rows=rows, n_q_heads=hq, n_kv_heads=hkv, head_dim=hd)
         s["work"] = torch.empty(max(16, s["work_bytes"]), dtype=torch.uint8, device="cuda")
     return s
 
@@ -288,8 +288,8 @@ def own_run(s):
     if case["op"] == "tree":
         import lokal_b200
         context().tree_attn(s["pool"], s["q"], s["out"], k_store=0, v_store=1, slots=s["slots"], q_start=s["q_start"], n_seqs=s["seqs"],
-                            rows=s["rows"], max_drafts=s["max_drafts"], mask=s["mask"], mask_words=s["words"], n_q_heads=s["hq"],
-                            n_kv_heads=s["hkv"], head_dim=s["hd"], scale=s["scale"], dtype=lokal_b200.dtype_id(s["q"]),
+                            rows=s["rows"], mask=s["mask"], mask_words=s["words"], n_q_heads=s["hq"], n_kv_heads=s["hkv"], head_dim=s["hd"],
+                             scale=s["scale"], dtype=lokal_b200.dtype_id(s["q"]),
                             kv_dtype=lokal_b200.dtype_id(s["k"]), workspace=s["work"], workspace_bytes=s["work_bytes"], stream=stream)
         return s["out"]
     s["book"].copy_(s["book0"])
@@ -297,7 +297,7 @@ def own_run(s):
         s["pool"].fork(s["src"], s["dst"], n=s["src"].numel(), stream=stream)
         s["pool"].reserve(s["every"], s["room"], n=s["every"].numel(), stream=stream)
     elif case["op"] == "accept":
-        s["pool"].tree_accept(s["slots"], s["q_start"], s["accepted"], s["counts"], n_seqs=case["seqs"], max_accept=case["per"], stream=stream)
+        s["pool"].accept(s["slots"], s["q_start"], s["accepted"], s["counts"], n_seqs=case["seqs"], max_accept=case["per"], stream=stream)
     else:
         s["pool"].compact(stream=stream)
     return kept(s)
