@@ -3,8 +3,9 @@
  * per-token layer ops: residual-add + RMSNorm (incl. per-head qk-norm), RoPE of
  * q/k with the bias fold, SiLU(gate)*up, and embedding gather with GGUF row
  * dequantisation (every block type the reference decodes) -- plus the steps
- * either side of that path: K/V staging into the cache, the gated-deltanet
- * per-row ops, and a GGUF container reader.
+ * either side of that path: K/V staging into the cache, a cache in pages and
+ * the attention of drafted rows over it, the gated-deltanet per-row ops, and a
+ * GGUF container reader.
  *
  * This is the boundary a `-b cuda` backend of the reference binds through FFI:
  * plain pointers and sizes, no C++ or framework types. Each entry point names
@@ -56,7 +57,10 @@ typedef enum lokal_status {
     LOKAL_ERR_IO = 8,          /* a file could not be opened or mapped */
     LOKAL_ERR_FORMAT = 9,      /* a GGUF file is malformed, truncated or of an unsupported version */
     LOKAL_ERR_NOT_FOUND = 10,  /* a tensor name or metadata key is not in the file */
-    LOKAL_ERR_POS_RANGE = 11   /* a position was negative or beyond the KV cache (its row was not stored) */
+    LOKAL_ERR_POS_RANGE = 11,  /* a position was negative or beyond the KV cache (its row was not stored) */
+    LOKAL_ERR_NO_PAGES = 12,   /* a cache pool had too few free pages (the entries that did not fit were skipped) */
+    LOKAL_ERR_PAGE_RANGE = 13  /* a slot, page, length or drafted row of a pool call was out of range or named twice
+                                  (its entry was skipped) */
 } lokal_status;
 
 /* GGUF tensor type ids (src/gguf/dequant.rs:21-41; BF16 = 30 per ggml.h).
@@ -351,6 +355,110 @@ LOKAL_API int lokal_cuda_kv_rows(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const
 LOKAL_API int lokal_cuda_kv_stage(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const void* src, int src_dtype,
                                   size_t src_row_stride, void* dst, int dst_dtype, size_t dst_row_stride,
                                   const uint32_t* dst_rows, size_t rows, size_t width);
+
+/* ---- A K/V cache in pages ---------------------------------------------------------------
+ * (No counterpart in the reference, whose cache is one linear region per slot, or a sink + ring: a sequence that
+ * continues another one is prefilled again there.) A pool groups the rows of a cache into pages, so that slots can
+ * share them, grow by them and give them back.
+ *
+ * `stores` are the cache buffers themselves, usually one for K and one for V of every layer, each n_pages * page_rows
+ * rows of row_bytes; page p is rows [p * page_rows, (p + 1) * page_rows) of every store. Three int32 arrays in device
+ * memory, the caller's like the stores, hold the state:
+ *   table [n_slots][max_pages]  page of positions [i * page_rows, (i + 1) * page_rows) of a slot, -1 = none
+ *   lens  [n_slots]             positions the slot holds
+ *   refs  [n_pages]             table entries that name the page; 0 = free
+ * lokal_cuda_kv_pool_reset makes them those of an empty pool; a program may also fill them itself, or save and restore
+ * them, as long as every slot has the pages of its lens positions and refs counts them. (A linear cache is the table
+ * [slot][i] = slot * max_pages + i with every refs 1.)
+ *
+ * Lists (slots, lengths, pages) are device arrays: a decode loop can run these calls with no host round trip and inside
+ * a captured graph; no call allocates. The calls on one pool read and rewrite its state and share its scratch memory:
+ * issue them in one order (one stream, or streams ordered by events). Results depend only on the state and the lists:
+ * new pages are the lowest-numbered free ones, in list order. An entry that cannot be carried out (a slot out of range
+ * or named by an earlier entry, a length the table cannot hold, no free page) is left undone, the others are not, and
+ * the next lokal_cuda_stream_sync returns LOKAL_ERR_PAGE_RANGE or LOKAL_ERR_NO_PAGES.
+ *
+ * page_rows: a power of two, 8 to 256. n_pages * page_rows and max_pages * page_rows at most 2^31 - 1. row_bytes even;
+ * with stores and row_bytes multiples of 16 bytes, copies use 16-byte accesses. A list has at most n_slots entries
+ * (and 65535). `stores` is a host array of device addresses. create and destroy allocate and free: not during a capture. */
+typedef struct lokal_kv_pool lokal_kv_pool;
+LOKAL_API int lokal_cuda_kv_pool_create(lokal_cuda_ctx* ctx, uint32_t page_rows, uint32_t n_pages, uint32_t n_slots, uint32_t max_pages,
+                                        int32_t* table, int32_t* lens, int32_t* refs, void* const* stores, uint32_t n_stores,
+                                        size_t row_bytes, lokal_kv_pool** out);
+LOKAL_API int lokal_cuda_kv_pool_destroy(lokal_cuda_ctx* ctx, lokal_kv_pool* pool);
+LOKAL_API int lokal_cuda_kv_pool_reset(lokal_cuda_ctx* ctx, lokal_cuda_stream s, lokal_kv_pool* pool);
+/* lokal_cuda_kv_rows for a pool: cache row of every token row (page * page_rows + offset), for lokal_cuda_kv_stage and
+ * the k_out_rows of lokal_cuda_qk_rope. A position the slot does not hold (reserve it first) gets LOKAL_KV_ROW_NONE and
+ * LOKAL_ERR_POS_RANGE. */
+LOKAL_API int lokal_cuda_kv_pool_rows(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const lokal_kv_pool* pool, const int32_t* positions,
+                                      int64_t pos0, const uint32_t* slots, uint32_t slot0, size_t rows, uint32_t* rows_out);
+/* Slot slots[i] grows to new_lens[i] positions (a smaller or equal length changes nothing). If it is going to write into
+ * a partly filled page that other slots hold too, it gets a copy of that page. When pages run out, the first entry that
+ * does not fit and those after it that need pages are left undone. */
+LOKAL_API int lokal_cuda_kv_pool_reserve(lokal_cuda_ctx* ctx, lokal_cuda_stream s, lokal_kv_pool* pool, const uint32_t* slots,
+                                         const int32_t* new_lens, size_t n);
+/* Slot dst_slots[i], which has to be empty, becomes a copy of slot src_slots[i] as it was before the call: it shares the
+ * full pages and gets a copy of the partly filled one. A source may be named any number of times. */
+LOKAL_API int lokal_cuda_kv_pool_fork(lokal_cuda_ctx* ctx, lokal_cuda_stream s, lokal_kv_pool* pool, const uint32_t* src_slots,
+                                      const uint32_t* dst_slots, size_t n);
+/* Slot slots[i] is cut to new_lens[i] positions (0 for all with new_lens NULL) and gives back the pages behind them; a
+ * page nobody holds any more is free. A larger length changes nothing. Here a slot may be named twice: the smallest
+ * length holds. */
+LOKAL_API int lokal_cuda_kv_pool_truncate(lokal_cuda_ctx* ctx, lokal_cuda_stream s, lokal_kv_pool* pool, const uint32_t* slots,
+                                          const int32_t* new_lens, size_t n);
+/* Moves pages down so that the used ones are 0 .. n_used - 1 (the free ones below n_used, ascending, take the used ones at
+ * or above it, ascending) and rewrites table and refs. n_used: device int32 or NULL. */
+LOKAL_API int lokal_cuda_kv_pool_compact(lokal_cuda_ctx* ctx, lokal_cuda_stream s, lokal_kv_pool* pool, int32_t* n_used);
+/* Page dst_pages[i] of every store gets the contents of page src_pages[i]; table and refs stay as they are. The targets
+ * have to be distinct and none of them a source. */
+LOKAL_API int lokal_cuda_kv_pool_copy_pages(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const lokal_kv_pool* pool, const int32_t* src_pages,
+                                            const int32_t* dst_pages, size_t n);
+/* After drafted rows have been verified (see lokal_cuda_tree_attn: the last q_start[i + 1] - q_start[i] positions of slot
+ * slots[i], or slot i with slots NULL): the rows of the accepted path, accepted[i][0 .. n_accepted[i]) in ascending
+ * order, move up behind the committed ones in every store, and the slot is cut behind them. accepted is
+ * [n_seqs][max_accept], max_accept at most 256. A sequence with a bad list is left as it was. */
+LOKAL_API int lokal_cuda_kv_pool_accept(lokal_cuda_ctx* ctx, lokal_cuda_stream s, lokal_kv_pool* pool, const uint32_t* slots,
+                                        const int32_t* q_start, const int32_t* accepted, const int32_t* n_accepted, uint32_t max_accept,
+                                        size_t n_seqs);
+
+/* ---- Attention of drafted rows over a pool ------------------------------------------------
+ * The reference's attention (src/model.rs, between the rotations and the output projection) reads the rows it staged one
+ * token at a time or as a causal chunk. Here a step may hold, per sequence, a tree of drafted tokens to verify at once
+ * (speculative decoding); one row per sequence is plain decoding, a chain is a causal chunk.
+ *
+ * Sequence i has rows [q_start[i], q_start[i + 1]) of the call (device int32[n_seqs + 1]; rows of the call that belong to
+ * no sequence are neither read nor written) and is slot slots[i] (slot i with slots NULL). Its n rows are the LAST n of
+ * the slot's positions: reserve them, stage their K and V (lokal_cuda_kv_stage, lokal_cuda_qk_rope with k_out_rows), then
+ * attend. The c = lens[slot] - n positions before them are committed.
+ *
+ * lokal_cuda_tree_plan fills what the rows need, each output optional: from parents (device int32[rows], the number of the
+ * parent within the sequence, smaller than the row's own, or -1 for a child of the last committed row; NULL = a chain)
+ *   mask[r][mask_words]  bit u of word u / 64: the row sees drafted row u (its ancestors and itself)
+ *   positions[r]         c + depth, for the rotation (depth 0 for a child of the last committed row)
+ *   cache_rows[r]        row of the stores that the row's K and V go to
+ * A parent out of range counts as -1 and is reported as LOKAL_ERR_PAGE_RANGE, as is a mask that is too narrow. */
+LOKAL_API int lokal_cuda_tree_plan(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const lokal_kv_pool* pool, const uint32_t* slots,
+                                   const int32_t* q_start, size_t n_seqs, size_t rows, const int32_t* parents, uint64_t* mask,
+                                   uint32_t mask_words, int32_t* positions, uint32_t* cache_rows);
+/* Bytes of workspace lokal_cuda_tree_attn needs on this context's GPU, at most, whatever the lengths (0 for sizes it refuses). */
+LOKAL_API size_t lokal_cuda_tree_attn_workspace(const lokal_cuda_ctx* ctx, size_t rows, uint32_t n_q_heads, uint32_t n_kv_heads,
+                                                uint32_t head_dim);
+/* Query head h of row j reads key head h / (n_q_heads / n_kv_heads) of its sequence:
+ *   z_t = scale * q . k_t,   out = sum_t exp(z_t) v_t / sum_t exp(z_t)
+ * over the committed positions and, of the drafted ones, those its mask names; mask NULL = those up to itself. Drafted
+ * rows past 64 * mask_words are not seen. A row that sees nothing gets zeros; what a row does not see does not reach it,
+ * infinities and NaN included, and rows of a page behind the slot's last position may hold anything.
+ * k_store, v_store: numbers of the pool's stores; their rows start with n_kv_heads * head_dim elements of kv_dtype.
+ * q, out: [rows][n_q_heads * head_dim] of dtype at the given row strides (elements); out must not overlap q.
+ * Types F32 / F16 / BF16, any of them for either; scores, maxima and sums are f32, and so are the products unless q and
+ * the cache have the same 16-bit type, where the tensor cores take the weights rounded to that type. head_dim up to 256.
+ * workspace: device memory, 16-byte aligned, of lokal_cuda_tree_attn_workspace bytes, used until the call is done: calls
+ * that may overlap need one each. Nothing of it has to be kept or cleared between calls. */
+LOKAL_API int lokal_cuda_tree_attn(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const lokal_kv_pool* pool, uint32_t k_store, uint32_t v_store,
+                                   const uint32_t* slots, const int32_t* q_start, size_t n_seqs, size_t rows, const uint64_t* mask,
+                                   uint32_t mask_words, const void* q, size_t q_row_stride, void* out, size_t out_row_stride,
+                                   uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t head_dim, float scale, int dtype, int kv_dtype,
+                                   void* workspace, size_t workspace_bytes);
 
 /* ---- Per-row siblings in the gated-deltanet (qwen35) blocks ----------------------
  * The same shape of work as the ops above (one pass over token rows), used by the

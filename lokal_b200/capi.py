@@ -25,13 +25,14 @@ PASS_SCHEDULE_AUTO, PASS_SCHEDULE_SEQUENTIAL, PASS_SCHEDULE_BRANCHES = 0, 1, 3
 
 # lokal_status
 OK, ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_MISALIGNED, ERR_CUDA, ERR_ID_RANGE, ERR_TIMEOUT, ERR_NO_DEVICE = range(8)
-ERR_IO, ERR_FORMAT, ERR_NOT_FOUND, ERR_POS_RANGE = 8, 9, 10, 11
+ERR_IO, ERR_FORMAT, ERR_NOT_FOUND, ERR_POS_RANGE, ERR_NO_PAGES, ERR_PAGE_RANGE = 8, 9, 10, 11, 12, 13
 KV_ROW_NONE = 0xFFFFFFFF
 STATUS_NAMES = {
     OK: "LOKAL_OK", ERR_BAD_ARG: "LOKAL_ERR_BAD_ARG", ERR_UNSUPPORTED: "LOKAL_ERR_UNSUPPORTED",
     ERR_MISALIGNED: "LOKAL_ERR_MISALIGNED", ERR_CUDA: "LOKAL_ERR_CUDA", ERR_ID_RANGE: "LOKAL_ERR_ID_RANGE",
     ERR_TIMEOUT: "LOKAL_ERR_TIMEOUT", ERR_NO_DEVICE: "LOKAL_ERR_NO_DEVICE", ERR_IO: "LOKAL_ERR_IO",
     ERR_FORMAT: "LOKAL_ERR_FORMAT", ERR_NOT_FOUND: "LOKAL_ERR_NOT_FOUND", ERR_POS_RANGE: "LOKAL_ERR_POS_RANGE",
+    ERR_NO_PAGES: "LOKAL_ERR_NO_PAGES", ERR_PAGE_RANGE: "LOKAL_ERR_PAGE_RANGE",
 }
 
 
@@ -136,6 +137,20 @@ SIGNATURES = {
     "lokal_cuda_window_write_spans": (_i, [C.POINTER(KvLayout), C.c_uint64, C.c_uint64, C.POINTER(C.c_uint64)]),
     "lokal_cuda_kv_rows": (_i, [_vp, _vp, C.POINTER(KvLayout), _vp, _i64, _vp, _u32, _sz, _vp]),
     "lokal_cuda_kv_stage": (_i, [_vp, _vp, _vp, _i, _sz, _vp, _i, _sz, _vp, _sz, _sz]),
+    "lokal_cuda_kv_pool_create": (_i, [_vp, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _u32, _sz, _pp]),
+    "lokal_cuda_kv_pool_destroy": (_i, [_vp, _vp]),
+    "lokal_cuda_kv_pool_reset": (_i, [_vp, _vp, _vp]),
+    "lokal_cuda_kv_pool_rows": (_i, [_vp, _vp, _vp, _vp, _i64, _vp, _u32, _sz, _vp]),
+    "lokal_cuda_kv_pool_reserve": (_i, [_vp, _vp, _vp, _vp, _vp, _sz]),
+    "lokal_cuda_kv_pool_fork": (_i, [_vp, _vp, _vp, _vp, _vp, _sz]),
+    "lokal_cuda_kv_pool_truncate": (_i, [_vp, _vp, _vp, _vp, _vp, _sz]),
+    "lokal_cuda_kv_pool_compact": (_i, [_vp, _vp, _vp, _vp]),
+    "lokal_cuda_kv_pool_copy_pages": (_i, [_vp, _vp, _vp, _vp, _vp, _sz]),
+    "lokal_cuda_kv_pool_accept": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _sz]),
+    "lokal_cuda_tree_plan": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _sz, _vp, _vp, _u32, _vp, _vp]),
+    "lokal_cuda_tree_attn_workspace": (_sz, [_vp, _sz, _u32, _u32, _u32]),
+    "lokal_cuda_tree_attn": (_i, [_vp, _vp, _vp, _u32, _u32, _vp, _vp, _sz, _sz, _vp, _u32, _vp, _sz, _vp, _sz, _u32, _u32, _u32, _f, _i, _i,
+                                  _vp, _sz]),
     "lokal_cuda_l2norm_rows": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _f, _i]),
     "lokal_cuda_gated_output_norm": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _f, _i, _i]),
     "lokal_cuda_attn_out_gate": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _i]),

@@ -29,7 +29,7 @@ namespace lokal {
 constexpr int kSmCountB200 = 148;
 
 // Device-side error word bits (read back by lokal_cuda_stream_sync).
-enum : unsigned { kErrIdRange = 1u, kErrTimeout = 2u, kErrPosRange = 4u };
+enum : unsigned { kErrIdRange = 1u, kErrTimeout = 2u, kErrPosRange = 4u, kErrNoPages = 8u, kErrPageRange = 16u };
 
 }  // namespace lokal
 

@@ -222,6 +222,26 @@ class Context:
                                                   dst_dtype, width if dst_row_stride is None else dst_row_stride,
                                                   _ptr(dst_rows), rows, width))
 
+    # -- drafted rows over a paged cache (KvPool) -----------------------------------
+    def tree_plan(self, pool, *, q_start, n_seqs, rows, slots=None, parents=None, mask=None, mask_words=0, positions=None, cache_rows=None,
+                  stream=None):
+        """From the parents of drafted rows (None: chains) their masks, rotation positions and cache rows (each optional)."""
+        self._check(self._lib.lokal_cuda_tree_plan(self._h, stream, pool.handle, _ptr(slots), _ptr(q_start), n_seqs, rows, _ptr(parents),
+                                                   _ptr(mask), mask_words, _ptr(positions), _ptr(cache_rows)))
+
+    def tree_attn_workspace(self, *, rows, n_q_heads, n_kv_heads, head_dim) -> int:
+        """Bytes of workspace tree_attn needs."""
+        return int(self._lib.lokal_cuda_tree_attn_workspace(self._h, rows, n_q_heads, n_kv_heads, head_dim))
+
+    def tree_attn(self, pool, q, out, *, k_store, v_store, q_start, n_seqs, rows, n_q_heads, n_kv_heads, head_dim, scale, dtype, kv_dtype,
+                  workspace, workspace_bytes, slots=None, mask=None, mask_words=0, q_row_stride=None, out_row_stride=None, stream=None):
+        """Attention of the last rows of each sequence's slot (drafted trees, chains, single tokens) over the pool's stores."""
+        width = n_q_heads * head_dim
+        self._check(self._lib.lokal_cuda_tree_attn(
+            self._h, stream, pool.handle, k_store, v_store, _ptr(slots), _ptr(q_start), n_seqs, rows, _ptr(mask), mask_words, _ptr(q),
+            width if q_row_stride is None else q_row_stride, _ptr(out), width if out_row_stride is None else out_row_stride, n_q_heads,
+            n_kv_heads, head_dim, scale, dtype, kv_dtype, _ptr(workspace), workspace_bytes))
+
     # -- per-row siblings in the gated-deltanet blocks ------------------------------
     def l2norm_rows(self, x, y=None, *, dim, eps, rows_per_token, n_tokens=1, tok_stride=0, dtype=F32, stream=None):
         """deltanet_ref::l2_norm over rows: y = x / max(sqrt(sum x^2), eps); in place when y is None."""
@@ -298,6 +318,73 @@ class Context:
         self._check(self._lib.lokal_cuda_host_embed_gather(self._h, _ptr(table_dev), ggml_type, vocab, dim, _ptr(ids),
                                                            ids.size, _ptr(out)))
         return out
+
+
+class KvPool:
+    """One `lokal_kv_pool`: the pages of a cache, and which slot holds which of them.
+
+    `table` (int32 [n_slots, max_pages]), `lens` (int32 [n_slots]), `refs` (int32 [n_pages]) and the stores are the caller's
+    device buffers; lists of slots, lengths and pages are device arrays too (int32 / uint32).
+    """
+
+    def __init__(self, ctx: Context, *, page_rows, n_pages, n_slots, max_pages, table, lens, refs, stores, row_bytes):
+        self.ctx = ctx
+        self._lib = ctx._lib
+        self._keep = (table, lens, refs, list(stores))
+        addrs = (C.c_void_p * len(stores))(*[_ptr(s) for s in stores])
+        h = C.c_void_p()
+        ctx._check(self._lib.lokal_cuda_kv_pool_create(ctx._h, page_rows, n_pages, n_slots, max_pages, _ptr(table), _ptr(lens), _ptr(refs),
+                                                       addrs, len(stores), row_bytes, C.byref(h)))
+        self._h = h
+
+    @property
+    def handle(self):
+        return self._h
+
+    def close(self):
+        if getattr(self, "_h", None) and self.ctx._h:
+            self._lib.lokal_cuda_kv_pool_destroy(self.ctx._h, self._h)
+        self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def reset(self, stream=None):
+        """Every slot empty, every page free."""
+        self.ctx._check(self._lib.lokal_cuda_kv_pool_reset(self.ctx._h, stream, self._h))
+
+    def rows(self, rows_out, *, rows, positions=None, pos0=0, slots=None, slot0=0, stream=None):
+        """Cache row of every token row into a device uint32 array (the paged twin of Context.kv_rows)."""
+        self.ctx._check(self._lib.lokal_cuda_kv_pool_rows(self.ctx._h, stream, self._h, _ptr(positions), pos0, _ptr(slots), slot0, rows,
+                                                          _ptr(rows_out)))
+
+    def reserve(self, slots, new_lens, *, n, stream=None):
+        """Slots grow to new_lens positions; a shared, partly filled last page is copied first."""
+        self.ctx._check(self._lib.lokal_cuda_kv_pool_reserve(self.ctx._h, stream, self._h, _ptr(slots), _ptr(new_lens), n))
+
+    def fork(self, src_slots, dst_slots, *, n, stream=None):
+        """Empty slots become copies of others: full pages shared, the partly filled one copied."""
+        self.ctx._check(self._lib.lokal_cuda_kv_pool_fork(self.ctx._h, stream, self._h, _ptr(src_slots), _ptr(dst_slots), n))
+
+    def truncate(self, slots, new_lens=None, *, n, stream=None):
+        """Slots are cut to new_lens positions (None: to none) and give back the pages behind them."""
+        self.ctx._check(self._lib.lokal_cuda_kv_pool_truncate(self.ctx._h, stream, self._h, _ptr(slots), _ptr(new_lens), n))
+
+    def compact(self, n_used=None, stream=None):
+        """Used pages move down to 0 .. n_used - 1."""
+        self.ctx._check(self._lib.lokal_cuda_kv_pool_compact(self.ctx._h, stream, self._h, _ptr(n_used)))
+
+    def copy_pages(self, src_pages, dst_pages, *, n, stream=None):
+        """Contents of whole pages, in every store."""
+        self.ctx._check(self._lib.lokal_cuda_kv_pool_copy_pages(self.ctx._h, stream, self._h, _ptr(src_pages), _ptr(dst_pages), n))
+
+    def accept(self, slots, q_start, accepted, n_accepted, *, n_seqs, max_accept, stream=None):
+        """The accepted drafted rows of each sequence move up behind the committed ones; the slot is cut behind them."""
+        self.ctx._check(self._lib.lokal_cuda_kv_pool_accept(self.ctx._h, stream, self._h, _ptr(slots), _ptr(q_start), _ptr(accepted),
+                                                            _ptr(n_accepted), max_accept, n_seqs))
 
 
 class LayerPass:

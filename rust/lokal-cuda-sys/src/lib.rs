@@ -25,6 +25,8 @@ pub const LOKAL_ERR_IO: c_int = 8;
 pub const LOKAL_ERR_FORMAT: c_int = 9;
 pub const LOKAL_ERR_NOT_FOUND: c_int = 10;
 pub const LOKAL_ERR_POS_RANGE: c_int = 11;
+pub const LOKAL_ERR_NO_PAGES: c_int = 12;
+pub const LOKAL_ERR_PAGE_RANGE: c_int = 13;
 
 // ---- lokal_type: the GgmlType discriminants (src/gguf/dequant.rs:21-41), so `ty as c_int` of a GgmlType works ----
 pub const LOKAL_F32: c_int = 0;
@@ -90,6 +92,8 @@ pub struct LokalCudaPass {
 }
 /// `lokal_cuda_stream`: a `cudaStream_t`; null is the default stream. One per `Session` / `Batcher`.
 pub type LokalCudaStream = *mut c_void;
+/// The pages of a K/V cache (`lokal_cuda_kv_pool_create`); only ever behind a pointer.
+pub type LokalKvPool = c_void;
 
 // ---- struct mirrors ----
 /// `lokal_qk_rope_params`: one fused bias + per-head RMSNorm + rotation call. Head geometry is explicit
@@ -258,6 +262,36 @@ pub fn lokal_cuda_create(device: c_int, out: *mut *mut LokalCudaCtx) -> c_int;
     pub fn lokal_cuda_kv_stage(ctx: *mut LokalCudaCtx, s: LokalCudaStream, src: *const c_void, src_dtype: c_int,
         src_row_stride: usize, dst: *mut c_void, dst_dtype: c_int, dst_row_stride: usize, dst_rows: *const u32,
         rows: usize, width: usize) -> c_int;
+    pub fn lokal_cuda_kv_pool_create(ctx: *mut LokalCudaCtx, page_rows: u32, n_pages: u32, n_slots: u32,
+        max_pages: u32, table: *mut i32, lens: *mut i32, refs: *mut i32, stores: *const *mut c_void, n_stores: u32,
+        row_bytes: usize, out: *mut *mut LokalKvPool) -> c_int;
+    pub fn lokal_cuda_kv_pool_destroy(ctx: *mut LokalCudaCtx, pool: *mut LokalKvPool) -> c_int;
+    pub fn lokal_cuda_kv_pool_reset(ctx: *mut LokalCudaCtx, s: LokalCudaStream, pool: *mut LokalKvPool) -> c_int;
+    pub fn lokal_cuda_kv_pool_rows(ctx: *mut LokalCudaCtx, s: LokalCudaStream, pool: *const LokalKvPool,
+        positions: *const i32, pos0: i64, slots: *const u32, slot0: u32, rows: usize, rows_out: *mut u32) -> c_int;
+    pub fn lokal_cuda_kv_pool_reserve(ctx: *mut LokalCudaCtx, s: LokalCudaStream, pool: *mut LokalKvPool,
+        slots: *const u32, new_lens: *const i32, n: usize) -> c_int;
+    pub fn lokal_cuda_kv_pool_fork(ctx: *mut LokalCudaCtx, s: LokalCudaStream, pool: *mut LokalKvPool,
+        src_slots: *const u32, dst_slots: *const u32, n: usize) -> c_int;
+    pub fn lokal_cuda_kv_pool_truncate(ctx: *mut LokalCudaCtx, s: LokalCudaStream, pool: *mut LokalKvPool,
+        slots: *const u32, new_lens: *const i32, n: usize) -> c_int;
+    pub fn lokal_cuda_kv_pool_compact(ctx: *mut LokalCudaCtx, s: LokalCudaStream, pool: *mut LokalKvPool,
+        n_used: *mut i32) -> c_int;
+    pub fn lokal_cuda_kv_pool_copy_pages(ctx: *mut LokalCudaCtx, s: LokalCudaStream, pool: *const LokalKvPool,
+        src_pages: *const i32, dst_pages: *const i32, n: usize) -> c_int;
+    pub fn lokal_cuda_kv_pool_accept(ctx: *mut LokalCudaCtx, s: LokalCudaStream, pool: *mut LokalKvPool,
+        slots: *const u32, q_start: *const i32, accepted: *const i32, n_accepted: *const i32, max_accept: u32,
+        n_seqs: usize) -> c_int;
+    pub fn lokal_cuda_tree_plan(ctx: *mut LokalCudaCtx, s: LokalCudaStream, pool: *const LokalKvPool,
+        slots: *const u32, q_start: *const i32, n_seqs: usize, rows: usize, parents: *const i32, mask: *mut u64,
+        mask_words: u32, positions: *mut i32, cache_rows: *mut u32) -> c_int;
+    pub fn lokal_cuda_tree_attn_workspace(ctx: *const LokalCudaCtx, rows: usize, n_q_heads: u32, n_kv_heads: u32,
+        head_dim: u32) -> usize;
+    pub fn lokal_cuda_tree_attn(ctx: *mut LokalCudaCtx, s: LokalCudaStream, pool: *const LokalKvPool, k_store: u32,
+        v_store: u32, slots: *const u32, q_start: *const i32, n_seqs: usize, rows: usize, mask: *const u64,
+        mask_words: u32, q: *const c_void, q_row_stride: usize, out: *mut c_void, out_row_stride: usize,
+        n_q_heads: u32, n_kv_heads: u32, head_dim: u32, scale: f32, dtype: c_int, kv_dtype: c_int,
+        workspace: *mut c_void, workspace_bytes: usize) -> c_int;
     pub fn lokal_cuda_l2norm_rows(ctx: *mut LokalCudaCtx, s: LokalCudaStream, x: *const c_void, y: *mut c_void,
         rows_per_token: usize, n_tokens: usize, tok_stride: usize, dim: usize, eps: f32, dtype: c_int) -> c_int;
     pub fn lokal_cuda_gated_output_norm(ctx: *mut LokalCudaCtx, s: LokalCudaStream, o: *const c_void,

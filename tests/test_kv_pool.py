@@ -1,0 +1,289 @@
+"""The pages of a K/V cache: fork, reserve, truncate, accept, compact and copy against a model that does one thing after the
+other in numpy. Integers and copied rows have to be equal bit for bit."""
+import numpy as np
+import pytest
+
+import lokal_b200 as L
+from lokal_b200 import capi
+from paged import PoolModel
+
+
+# ---- no GPU ----
+
+def test_null_arguments_are_refused():
+    lib = capi.load()
+    out = (capi.C.c_void_p * 1)()
+    assert lib.lokal_cuda_kv_pool_create(None, 16, 1, 1, 1, None, None, None, None, 1, 16, out) == capi.ERR_BAD_ARG
+    for name in ("reset", "compact", "destroy"):
+        fn = getattr(lib, "lokal_cuda_kv_pool_" + name)
+        assert fn(*[None] * len(fn.argtypes)) == capi.ERR_BAD_ARG
+    for name in ("rows", "reserve", "fork", "truncate", "copy_pages", "accept"):
+        fn = getattr(lib, "lokal_cuda_kv_pool_" + name)
+        assert fn(*[0 if t in (capi.C.c_size_t, capi.C.c_uint32, capi.C.c_int64) else None for t in fn.argtypes]) == capi.ERR_BAD_ARG
+
+
+def test_model_shares_copies_and_frees():
+    m = PoolModel(8, 6, 3, 4, np.arange(2 * 48 * 1).reshape(2, 48, 1))
+    m.reserve([0], [13])
+    m.fork([0], [1])
+    assert m.table[1, 0] == m.table[0, 0] == 0 and m.table[1, 1] == 2 and list(m.refs[:3]) == [2, 1, 1]
+    assert (m.rows[:, 16:21] == m.rows[:, 8:13]).all()
+    m.truncate([0])
+    assert list(m.refs[:3]) == [1, 0, 1] and m.compact() == 2 and list(m.table[1, :2]) == [0, 1]
+    m.reserve([2], [33])
+    assert m.bad and not m.no_pages
+    m.reserve([2, 0], [32, 8])
+    assert not m.no_pages or m.lens[0] == 0
+
+
+# ---- GPU ----
+
+class Rig:
+    """A pool on the device beside its model."""
+
+    def __init__(self, ctx, dev, page, n_pages, n_slots, max_pages, n_stores, width, seed, shift=0):
+        import torch
+        self.torch, self.ctx = torch, ctx
+        rng = np.random.default_rng(seed)
+        rows = rng.integers(0, 65536, (n_stores, n_pages * page, width)).astype(np.uint16)
+        self.m = PoolModel(page, n_pages, n_slots, max_pages, rows.copy())
+        flat = torch.zeros(rows.size + 64, dtype=torch.int16, device="cuda")
+        self.store = flat[shift:shift + rows.size].view(rows.shape)
+        self.store.copy_(torch.from_numpy(rows.view(np.int16)))
+        self.table = torch.full((n_slots, max_pages), 7, dtype=torch.int32, device="cuda")
+        self.lens = torch.full((n_slots,), 7, dtype=torch.int32, device="cuda")
+        self.refs = torch.full((n_pages,), 7, dtype=torch.int32, device="cuda")
+        self.pool = L.KvPool(ctx, page_rows=page, n_pages=n_pages, n_slots=n_slots, max_pages=max_pages, table=self.table, lens=self.lens,
+                             refs=self.refs, stores=[self.store[i] for i in range(n_stores)], row_bytes=2 * width)
+        self.pool.reset()
+
+    def ints(self, a):
+        return self.torch.tensor(np.asarray(a, np.int64).astype(np.uint32).view(np.int32), device="cuda") if len(a) else \
+            self.torch.zeros(1, dtype=self.torch.int32, device="cuda")
+
+    def sync(self):
+        try:
+            self.ctx.stream_sync()
+            return capi.OK
+        except L.LokalCudaError as e:
+            return e.status
+
+    def same(self, what):
+        status = self.sync()
+        want = capi.ERR_NO_PAGES if self.m.no_pages else capi.ERR_PAGE_RANGE if self.m.bad else capi.OK
+        assert status == want, what
+        self.m.no_pages = self.m.bad = False
+        assert np.array_equal(self.lens.cpu().numpy(), self.m.lens), what
+        assert np.array_equal(self.table.cpu().numpy(), self.m.table), what
+        assert np.array_equal(self.refs.cpu().numpy(), self.m.refs), what
+        assert np.array_equal(self.store.cpu().numpy().view(np.uint16), self.m.rows), what
+        held = np.bincount(self.m.table[self.m.table >= 0], minlength=self.m.n_pages)
+        assert np.array_equal(held, self.m.refs), what
+
+    def both(self, name, *lists):
+        getattr(self.m, name)(*lists)
+        getattr(self.pool, name)(*[None if a is None else self.ints(a) for a in lists], n=len(lists[0]))
+
+    def accept(self, slots, n_rows, accepted, counts):
+        self.m.accept(slots, n_rows, accepted, counts)
+        starts = np.concatenate([[0], np.cumsum(n_rows)])
+        self.pool.accept(self.ints(slots), self.ints(starts), self.ints(np.asarray(accepted).reshape(-1)), self.ints(counts), n_seqs=len(slots),
+                         max_accept=np.asarray(accepted).shape[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page,n_pages,n_slots,max_pages,n_stores,width,shift", [
+    (8, 40, 9, 10, 4, 8, 0), (16, 300, 40, 12, 6, 72, 0), (64, 24, 7, 5, 2, 512, 0), (256, 9, 5, 3, 2, 24, 0),
+    (16, 60, 12, 9, 3, 5, 0),      # rows of ten bytes: no 16-byte accesses
+    (16, 60, 12, 9, 3, 16, 1),     # stores that are only 2-byte aligned
+    (8, 5000, 30, 400, 2, 8, 0),   # more pages than one pass of the plan's scan takes
+])
+def test_any_order_of_calls_matches_the_model(ctx, dev, page, n_pages, n_slots, max_pages, n_stores, width, shift):
+    r = Rig(ctx, dev, page, n_pages, n_slots, max_pages, n_stores, width, page + n_pages, shift)
+    rng = np.random.default_rng(n_pages)
+    r.same("empty")
+    cap = page * max_pages
+    for step in range(40):
+        name = rng.choice(["reserve", "reserve", "fork", "truncate", "accept", "compact"])
+        k = int(rng.integers(1, n_slots + 1))
+        slots = rng.permutation(n_slots)[:k]
+        if name == "reserve":
+            r.both("reserve", slots, np.minimum(cap, r.m.lens[slots] + rng.integers(0, 4 * page, k)))
+        elif name == "fork":
+            empty = np.flatnonzero(r.m.lens == 0)[:k]
+            if len(empty):
+                r.both("fork", rng.integers(0, n_slots, len(empty)), empty)
+        elif name == "truncate":
+            k = max(1, k // 3)
+            if rng.random() < 0.3:
+                r.both("truncate", slots[:k], None)
+            else:
+                r.both("truncate", slots[:k], (r.m.lens[slots[:k]] * rng.random(k)).astype(int))
+        elif name == "accept":
+            # rows may be moved only in pages that no other slot holds: grow first, as a program does before it drafts
+            drafts = rng.integers(0, 12, k)
+            want = np.minimum(cap, r.m.lens[slots] + drafts)
+            r.both("reserve", slots, want)
+            ok = r.m.lens[slots] == want
+            n = np.where(ok, drafts, 0)
+            n = np.minimum(n, r.m.lens[slots])
+            counts = np.array([rng.integers(0, x + 1) for x in n])
+            acc = np.zeros((k, 12), np.int64)
+            for i in range(k):
+                acc[i, :counts[i]] = np.sort(rng.permutation(n[i])[:counts[i]])
+            r.accept(slots, n, acc, counts)
+        else:
+            used = r.torch.zeros(1, dtype=r.torch.int32, device="cuda")
+            r.pool.compact(used)
+            assert r.m.compact() == int(used.item())
+        r.same(f"step {step}: {name}")
+
+
+@pytest.mark.gpu
+def test_accept_moves_rows_in_place_when_targets_are_later_sources(ctx, dev):
+    # the path 1, 2, 3, ... moves to 0, 1, 2, ...: every target is the next move's source; 31 moves cross pages and batches
+    for page in (8, 16):
+        r = Rig(ctx, dev, page, 12, 2, 8, 3, 40, page)
+        r.both("reserve", [1], [5 + 32])
+        r.accept([1], [32], [list(range(1, 32))], [31])
+        r.same("a chain shifted by one")
+        assert r.m.lens[1] == 36
+        r.accept([1], [4], [[0, 2]], [2])
+        r.same("the first stays")
+        r.accept([1], [3], [[0, 0]], [0])
+        r.same("none accepted")
+
+
+@pytest.mark.gpu
+def test_writers_of_a_shared_partly_filled_page_get_their_own(ctx, dev):
+    # a fork cut back into a page that its source still holds: whoever grows first takes a copy
+    r = Rig(ctx, dev, 16, 20, 4, 6, 2, 64, 3)
+    r.both("reserve", [0], [48])
+    r.both("fork", [0, 0], [1, 2])
+    r.both("truncate", [1, 2], [37, 41])
+    r.same("shared last page")
+    assert r.m.refs[r.m.table[0, 2]] == 3
+    r.both("reserve", [1, 2, 0], [40, 60, 48])
+    r.same("copied before it is written")
+    assert r.m.refs[r.m.table[0, 2]] == 1 and len({int(r.m.table[i, 2]) for i in range(3)}) == 3
+
+
+@pytest.mark.gpu
+def test_pages_run_out_in_list_order(ctx, dev):
+    r = Rig(ctx, dev, 8, 10, 6, 8, 2, 8, 5)
+    r.both("reserve", [0, 1, 2, 3, 4], [24, 40, 32, 8, 0])  # 3 + 5 fit, 4 do not, and the one after it is not served either
+    assert r.m.no_pages and list(r.m.lens[:5]) == [24, 40, 0, 0, 0]
+    r.same("exhausted")
+    r.both("truncate", [1, 1, 0], [17, 9, 50])  # the smaller of the two lengths of slot 1
+    r.same("given back")
+    assert r.m.lens[1] == 9 and r.m.lens[0] == 24
+    r.both("fork", [1, 1, 1, 1, 1, 1], [2, 3, 4, 5, 2, 9])  # slot 2 twice, and one that is not there
+    assert r.m.bad
+    r.same("forks")
+    r.both("truncate", [0, 1, 2, 3, 4, 5], None)
+    r.same("all freed")
+    assert not r.m.refs.any()
+
+
+@pytest.mark.gpu
+def test_bad_entries_change_nothing_and_are_reported(ctx, dev):
+    r = Rig(ctx, dev, 8, 12, 4, 4, 2, 8, 7)
+    r.both("reserve", [0, 1], [12, 20])
+    r.same("start")
+    for name, lists in [("reserve", ([9], [8])), ("reserve", ([0], [33])), ("reserve", ([0], [-1])), ("reserve", ([2, 2], [8, 16])),
+                        ("fork", ([0], [1])), ("fork", ([0], [0])), ("fork", ([7], [2])), ("truncate", ([4], [0])), ("truncate", ([0], [-5]))]:
+        r.both(name, *lists)
+        assert r.m.bad, (name, lists)
+        r.same(f"{name} {lists}")
+    for n, acc, count in [([4], [[2, 1]], [2]), ([4], [[1, 1]], [2]), ([4], [[0, 4]], [2]), ([4], [[-1, 2]], [2]), ([4], [[0, 1]], [5]),
+                          ([30], [[0, 1]], [2]), ([4], [[0, 1]], [-1])]:
+        r.accept([1], n, acc, count)
+        assert r.m.bad
+        r.same(f"accept {n} {acc} {count}")
+    r.accept([1, 1], [2, 2], [[1], [1]], [1, 1])
+    assert r.m.bad
+    r.same("one slot twice")
+
+
+@pytest.mark.gpu
+def test_pages_are_copied_and_rows_are_found(ctx, dev):
+    import torch
+    r = Rig(ctx, dev, 16, 40, 4, 6, 3, 24, 11)
+    src, dst = [0, 5, 39, 5], [10, 11, 12, 13]
+    r.pool.copy_pages(r.ints(src), r.ints(dst), n=4)
+    for a, b in zip(src, dst):
+        r.m._copy(a, b, 16)
+    r.same("copied")
+    r.pool.copy_pages(r.ints([0, 40]), r.ints([-1, 3]), n=2)
+    r.m.bad = True
+    r.same("pages that are not there")
+    r.both("reserve", [3, 1], [50, 17])
+    r.same("reserved")
+    pos = np.array([0, 15, 16, 49, 50, -1, 16, 17, 3], np.int32)
+    slots = np.array([3, 3, 3, 3, 3, 1, 1, 1, 8], np.uint32)
+    out = torch.zeros(9, dtype=torch.int32, device="cuda")
+    r.pool.rows(out, rows=9, positions=r.ints(pos), slots=r.ints(slots))
+    assert r.sync() == capi.ERR_POS_RANGE
+    want = [r.m.row(s, p) if s < 4 and 0 <= p < r.m.lens[s] else capi.KV_ROW_NONE for s, p in zip(slots, pos)]
+    assert np.array_equal(out.cpu().numpy().view(np.uint32), np.array(want, np.uint32))
+    r.pool.rows(out, rows=9, pos0=9, slot0=3)
+    assert r.sync() == capi.OK
+    assert list(out.cpu().numpy()) == [r.m.row(3, 9 + i) for i in range(9)]
+
+
+@pytest.mark.gpu
+def test_a_captured_step_replays_on_the_state_it_finds(ctx, dev):
+    r = Rig(ctx, dev, 8, 64, 8, 12, 2, 16, 13)
+    r.both("reserve", [0, 1], [13, 30])
+    r.same("start")
+    src, dst, grow, want, none = r.ints([0, 1]), r.ints([2, 3]), r.ints([2, 3]), r.ints([40, 41]), r.ints([0, 1])
+    s = ctx.stream_create()
+    ctx.graph_begin(s)
+    r.pool.fork(src, dst, n=2, stream=s)
+    r.pool.reserve(grow, want, n=2, stream=s)
+    r.pool.compact(stream=s)
+    graph = ctx.graph_end(s)
+    r.same("capturing changes nothing")
+    for cut in ([13, 30], [8, 17], [0, 1]):
+        ctx.graph_launch(graph, s)
+        ctx.stream_sync(s)
+        r.m.fork([0, 1], [2, 3])
+        r.m.reserve([2, 3], [40, 41])
+        r.m.compact()
+        r.same(f"replayed {cut}")
+        r.both("truncate", [2, 3], None)
+        r.both("truncate", [0, 1], cut)
+        r.same(f"cut {cut}")
+    ctx.graph_destroy(graph)
+    ctx.stream_destroy(s)
+
+
+@pytest.mark.gpu
+def test_create_refusals(ctx, dev):
+    import torch
+    t = torch.zeros(4096, dtype=torch.int32, device="cuda")
+    good = dict(page_rows=16, n_pages=4, n_slots=2, max_pages=2, table=t, lens=t[64:], refs=t[128:], stores=[t[256:]], row_bytes=16)
+    L.KvPool(ctx, **good).close()
+    for bad, status in [(dict(page_rows=4), capi.ERR_BAD_ARG), (dict(page_rows=24), capi.ERR_BAD_ARG), (dict(page_rows=512), capi.ERR_BAD_ARG),
+                        (dict(n_pages=0), capi.ERR_BAD_ARG), (dict(n_slots=0), capi.ERR_BAD_ARG), (dict(max_pages=0), capi.ERR_BAD_ARG),
+                        (dict(stores=[]), capi.ERR_BAD_ARG), (dict(row_bytes=0), capi.ERR_BAD_ARG), (dict(row_bytes=7), capi.ERR_BAD_ARG),
+                        (dict(n_pages=1 << 27), capi.ERR_BAD_ARG), (dict(max_pages=1 << 28), capi.ERR_BAD_ARG), (dict(table=None), capi.ERR_BAD_ARG),
+                        (dict(stores=[None]), capi.ERR_BAD_ARG), (dict(lens=t.data_ptr() + 2), capi.ERR_MISALIGNED),
+                        (dict(stores=[t.data_ptr() + 1]), capi.ERR_MISALIGNED)]:
+        with pytest.raises(L.LokalCudaError) as e:
+            L.KvPool(ctx, **{**good, **bad})
+        assert e.value.status == status, bad
+    pool = L.KvPool(ctx, **good)
+    for call in (lambda: pool.reserve(t, t, n=3), lambda: pool.reserve(t, None, n=1), lambda: pool.fork(None, t, n=1),
+                 lambda: pool.copy_pages(t, t, n=5), lambda: pool.accept(t, t, t, t, n_seqs=1, max_accept=257),
+                 lambda: pool.accept(t, t, None, t, n_seqs=1, max_accept=1), lambda: pool.rows(None, rows=1), lambda: pool.rows(t, rows=1, pos0=-1)):
+        with pytest.raises(L.LokalCudaError) as e:
+            call()
+        assert e.value.status == capi.ERR_BAD_ARG
+    with pytest.raises(L.LokalCudaError) as e:
+        pool.truncate(t.data_ptr() + 1, n=1)
+    assert e.value.status == capi.ERR_MISALIGNED
+    pool.reserve(None, None, n=0)
+    pool.fork(None, None, n=0)
+    ctx.stream_sync()
+    pool.close()

@@ -1,0 +1,525 @@
+"""Attention of drafted rows over a paged cache, and the plan that makes its masks, against a plain f64 form on the CPU.
+Tolerances are the bound of tests/paged.py::tolerance, element for element."""
+import numpy as np
+import pytest
+
+import lokal_b200 as L
+import synth
+from lokal_b200 import capi
+from paged import attention, tolerance, visible
+from synth import BF16, F16, F32
+
+
+def test_null_arguments_are_refused():
+    lib = capi.load()
+    for name in ("lokal_cuda_tree_plan", "lokal_cuda_tree_attn"):
+        fn = getattr(lib, name)
+        assert fn(*[None if t is capi.C.c_void_p else 0 for t in fn.argtypes]) == capi.ERR_BAD_ARG
+    assert lib.lokal_cuda_tree_attn_workspace(None, 1, 1, 1, 64) == 0
+
+
+def random_parents(rng, n):
+    return np.array([int(rng.integers(max(-1, j - 6), j)) for j in range(n)], np.int32)
+
+
+def mask_of(parents, words):
+    out = np.zeros((len(parents), words), np.uint64)
+    for j, p in enumerate(parents):
+        if p >= 0:
+            out[j] = out[p]
+        out[j, j // 64] |= np.uint64(1) << np.uint64(j % 64)
+    return out
+
+
+def bits(rows, words, rng):
+    return rng.integers(0, 2 ** 63, (rows, words)).astype(np.uint64) * np.uint64(2) + rng.integers(0, 2, (rows, words)).astype(np.uint64)
+
+
+class Case:
+    """Sequences of a pool, their rows and the cache, on both sides."""
+
+    def __init__(self, ctx, dev, *, lens, drafts, hq, hkv, hd, page=16, dtype=F32, kv=F32, mask="tree", seed=0, pad=0, q_pad=0, scale=None,
+                 k_scale=1.0, extra_rows=0, slots=None, spare=2):
+        import torch
+        self.torch, self.ctx, self.dev = torch, ctx, dev
+        rng = np.random.default_rng(seed)
+        self.lens, self.drafts = np.asarray(lens, np.int64), np.asarray(drafts, np.int64)
+        self.hq, self.hkv, self.hd, self.page, self.dtype, self.kv = hq, hkv, hd, page, dtype, kv
+        self.scale = hd ** -0.5 if scale is None else scale
+        n = len(lens)
+        self.slots = np.arange(n) if slots is None else np.asarray(slots)
+        held = -(-self.lens // page)
+        self.n_pages = int(held.sum()) + spare
+        self.max_pages = int(held.max()) + 1
+        self.n_slots = int(self.slots.max()) + 2
+        order = rng.permutation(self.n_pages)
+        self.table = np.full((self.n_slots, self.max_pages), -1, np.int32)
+        at = 0
+        for i in range(n):
+            self.table[self.slots[i], :held[i]] = order[at:at + held[i]]
+            at += held[i]
+        self.starts = np.concatenate([[0], np.cumsum(self.drafts)])
+        self.rows = int(self.starts[-1]) + extra_rows
+        self.width = hkv * hd + pad
+        self.k = synth.round_to(rng.standard_normal((self.n_pages * page, self.width), dtype=np.float32) * np.float32(k_scale), kv)
+        self.v = synth.round_to(rng.standard_normal((self.n_pages * page, self.width), dtype=np.float32), kv)
+        self.q = synth.round_to(rng.standard_normal((self.rows, hq * hd + q_pad), dtype=np.float32), dtype)
+        words = max(1, -(-int(self.drafts.max()) // 64))
+        self.mask = None
+        if mask == "tree":
+            self.mask = np.concatenate([mask_of(random_parents(rng, int(d)), words) for d in self.drafts] + [np.zeros((extra_rows, words), np.uint64)])
+        elif mask == "random":
+            self.mask = bits(self.rows, words, rng)
+        elif mask == "none":
+            self.mask = np.zeros((self.rows, words), np.uint64)
+        self.words = words
+        self.fill = 7.0
+
+    def cache_row(self, i, pos):
+        return self.table[self.slots[i], pos // self.page].astype(np.int64) * self.page + pos % self.page
+
+    def upload(self):
+        put, t = self.dev.put, self.torch
+        d = {"table": put(self.table), "k": put(self.k, self.kv), "v": put(self.v, self.kv), "q": put(self.q, self.dtype)}
+        lens = np.zeros(self.n_slots, np.int32)
+        lens[self.slots] = self.lens
+        d["lens"] = put(lens)
+        d["refs"] = t.zeros(self.n_pages, dtype=t.int32, device="cuda")
+        d["starts"] = put(self.starts.astype(np.int32))
+        d["slots"] = put(self.slots.astype(np.int32))
+        d["mask"] = None if self.mask is None else put(self.mask.view(np.int64))
+        d["out"] = self.dev.empty((self.rows, self.q.shape[1]), self.dtype, fill=self.fill)
+        d["bytes"] = self.ctx.tree_attn_workspace(rows=self.rows, n_q_heads=self.hq, n_kv_heads=self.hkv, head_dim=self.hd)
+        d["work"] = t.full((d["bytes"] + 64,), 255, dtype=t.uint8, device="cuda")  # NaN everywhere: nothing of it is read unwritten
+        d["pool"] = L.KvPool(self.ctx, page_rows=self.page, n_pages=self.n_pages, n_slots=self.n_slots, max_pages=self.max_pages, table=d["table"],
+                             lens=d["lens"], refs=d["refs"], stores=[d["k"], d["v"]], row_bytes=self.width * d["k"].element_size())
+        self.d = d
+        return d
+
+    def call(self, stream=None, **over):
+        d = self.d
+        kw = dict(k_store=0, v_store=1, slots=d["slots"], q_start=d["starts"], n_seqs=len(self.lens), rows=self.rows, mask=d["mask"],
+                  mask_words=self.words if d["mask"] is not None else 0, n_q_heads=self.hq, n_kv_heads=self.hkv, head_dim=self.hd, scale=self.scale,
+                  dtype=self.dtype, kv_dtype=self.kv, workspace=d["work"], workspace_bytes=d["bytes"], q_row_stride=self.q.shape[1],
+                  out_row_stride=self.q.shape[1], stream=stream)
+        self.ctx.tree_attn(d["pool"], d["q"], d["out"], **{**kw, **over})
+
+    def run(self):
+        self.upload()
+        self.call()
+        self.ctx.stream_sync()
+        return self.dev.get(self.d["out"])
+
+    def check(self, got, what=""):
+        g = self.hq // self.hkv
+        rounded = self.dtype == self.kv and self.dtype != F32
+        for i in range(len(self.lens)):
+            n, length = int(self.drafts[i]), int(self.lens[i])
+            if n == 0:
+                continue
+            r0 = int(self.starts[i])
+            see = visible(n, length - n, None if self.mask is None else self.mask[r0:r0 + n])
+            at = self.cache_row(i, np.arange(length))
+            for h in range(self.hq):
+                kc = slice((h // g) * self.hd, (h // g + 1) * self.hd)
+                qc = slice(h * self.hd, (h + 1) * self.hd)
+                out, size, terms = attention(self.q[r0:r0 + n, qc], self.k[at, kc], self.v[at, kc], see, np.float32(self.scale))
+                tol = tolerance(out, size, terms, length, self.hd, self.dtype, rounded)
+                err = np.abs(got[r0:r0 + n, qc] - out)
+                assert (err <= tol).all(), f"{what}: sequence {i}, head {h}: {err.max():.3e} against {tol.flat[np.argmax(err - tol)]:.3e}"
+        # nothing else is written: rows behind the last sequence, columns behind the heads
+        assert (got[int(self.starts[-1]):] == self.fill).all() and (got[:, self.hq * self.hd:] == self.fill).all(), what
+
+
+TYPES = [(F32, F32), (F32, F16), (F32, BF16), (F16, F16), (BF16, BF16), (F16, BF16), (BF16, F32)]
+RAGGED = dict(lens=[1, 2, 17, 64, 65, 129, 300, 1000], drafts=[1, 2, 5, 9, 1, 33, 12, 20])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv", TYPES)
+@pytest.mark.parametrize("hq,hkv,hd", [(4, 2, 64), (14, 2, 64), (4, 2, 128), (2, 1, 256)])
+def test_types_and_heads(ctx, dev, dtype, kv, hq, hkv, hd):
+    c = Case(ctx, dev, **RAGGED, hq=hq, hkv=hkv, hd=hd, dtype=dtype, kv=kv, seed=hq + hd)
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("hq,hkv,hd", [(3, 3, 40), (6, 2, 72), (5, 1, 80), (20, 1, 96), (34, 2, 64), (150, 1, 64), (2, 2, 1), (3, 1, 5), (1, 1, 130), (4, 4, 192)])
+def test_odd_head_sizes_and_groups(ctx, dev, dtype, hq, hkv, hd):
+    c = Case(ctx, dev, lens=[1, 40, 200], drafts=[1, 7, 30], hq=hq, hkv=hkv, hd=hd, dtype=dtype, kv=dtype, seed=hd)
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv", [(F32, F16), (BF16, BF16), (F16, F16)])
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 256])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_pages_that_end_anywhere_in_a_tile(ctx, dev, dtype, kv, page, hd):
+    c = Case(ctx, dev, lens=[page - 1, page, page + 1, 127, 128, 129, 255, 257, 640], drafts=[1, 1, 2, 3, 4, 5, 6, 65, 130], hq=4, hkv=2, hd=hd, page=page,
+             dtype=dtype, kv=kv, seed=page, slots=[3, 0, 7, 1, 2, 5, 4, 9, 6])
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv", [(F32, F32), (F32, F16), (BF16, BF16), (F16, F16)])
+@pytest.mark.parametrize("mask", ["chain", "random", "none"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_masks(ctx, dev, dtype, kv, mask, hd):
+    # "none": drafted rows that see no drafted row, and nothing at all where nothing is committed (rows of zeros)
+    c = Case(ctx, dev, lens=[3, 70, 100, 161, 260, 5], drafts=[3, 70, 63, 64, 97, 1], hq=6, hkv=2, hd=hd, dtype=dtype, kv=kv, mask=mask, seed=5)
+    got = c.run()
+    c.check(got)
+    if mask == "none":
+        assert (got[:73, :6 * hd] == 0.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv", [(F32, F16), (BF16, BF16)])
+def test_a_narrow_mask_hides_the_rows_it_has_no_bits_for(ctx, dev, dtype, kv):
+    c = Case(ctx, dev, lens=[200], drafts=[150], hq=2, hkv=1, hd=64, dtype=dtype, kv=kv, mask="random", seed=2)
+    c.mask, c.words = np.ascontiguousarray(c.mask[:, :1]), 1
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv", TYPES)
+def test_strides_and_rows_of_no_sequence(ctx, dev, dtype, kv):
+    c = Case(ctx, dev, lens=[50, 9, 300], drafts=[3, 0, 17], hq=4, hkv=2, hd=64, dtype=dtype, kv=kv, pad=24, q_pad=40, extra_rows=5, seed=8)
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_rows_and_stores_off_the_16_byte_grid(ctx, dev, dtype):
+    # strides that are odd, and a q that starts one element into its buffer
+    c = Case(ctx, dev, lens=[33, 200], drafts=[2, 9], hq=2, hkv=1, hd=64, dtype=dtype, kv=dtype, pad=2 if dtype == F32 else 1, q_pad=3, seed=9)
+    d = c.upload()
+    flat = c.torch.zeros(d["q"].numel() + 1, dtype=d["q"].dtype, device="cuda")
+    shifted = flat[1:].view(d["q"].shape)
+    shifted.copy_(d["q"])
+    d["q"] = shifted
+    c.call()
+    ctx.stream_sync()
+    c.check(dev.get(d["out"]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv,hd", [(F32, F16, 64), (BF16, BF16, 64), (BF16, BF16, 128), (F16, F16, 128), (F32, F32, 128)])
+def test_what_is_not_seen_does_not_reach_a_row(ctx, dev, dtype, kv, hd):
+    """Infinities and NaN in rows behind the last position, in pages nobody holds, and in drafted rows that only some see."""
+    c = Case(ctx, dev, lens=[150, 41, 300], drafts=[20, 9, 70], hq=4, hkv=2, hd=hd, dtype=dtype, kv=kv, mask="tree", seed=21)
+    clean = c.run()
+    c.check(clean)
+    used = np.zeros(c.n_pages * c.page, bool)
+    for i in range(3):
+        used[c.cache_row(i, np.arange(int(c.lens[i])))] = True
+    c.k[~used], c.v[~used] = np.nan, np.inf
+    again = c.run()
+    assert np.array_equal(again, clean), "rows that belong to nobody"
+    # a drafted row of sequences 0 and 2 goes bad: the rows that do not see it keep their results
+    for i, node, kbad, vbad in [(0, 4, 1.0, np.nan), (0, 7, np.nan, 1.0), (2, 30, np.inf, np.inf), (2, 66, 1.0, -np.inf)]:
+        row = c.cache_row(i, np.array([int(c.lens[i] - c.drafts[i]) + node]))[0]
+        k0, v0 = c.k[row].copy(), c.v[row].copy()
+        if kbad != 1.0:
+            c.k[row, 3::hd] = kbad
+        if vbad != 1.0:
+            c.v[row, 3::hd] = vbad
+        got = c.run()
+        c.k[row], c.v[row] = k0, v0
+        r0, n = int(c.starts[i]), int(c.drafts[i])
+        sees = visible(n, 0, c.mask[r0:r0 + n])[:, node]
+        rows = np.ones(c.rows, bool)
+        rows[r0:r0 + n] = ~sees
+        # same arithmetic but for the order in which a row's sums are taken: within the tolerance of either
+        good = got.copy()
+        good[~rows] = clean[~rows]
+        c.check(good, f"bad row {node} of sequence {i}")
+        hit = got[~rows].reshape(-1, c.hq, hd)
+        if vbad != 1.0:
+            assert not np.isfinite(hit[:, :, 3]).any()
+        if vbad != 1.0 and kbad == 1.0:  # a score of +inf makes the whole row inf - inf
+            keep = np.delete(hit, 3, axis=2)
+            assert np.isfinite(keep).all()
+            assert np.allclose(keep, np.delete(clean[~rows].reshape(-1, c.hq, hd), 3, axis=2), rtol=0.05, atol=0.05)
+        if np.isnan(kbad):
+            assert np.isnan(hit).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv,hd", [(F32, F16, 64), (F32, F32, 128), (BF16, BF16, 64), (BF16, BF16, 128), (F16, F16, 64)])
+def test_long_contexts_are_split_and_joined(ctx, dev, dtype, kv, hd):
+    # few rows over many keys: every block of rows is shared by many CTAs
+    c = Case(ctx, dev, lens=[20011, 3], drafts=[9, 1], hq=2, hkv=1, hd=hd, page=64, dtype=dtype, kv=kv, seed=31)
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv,hd", [(F32, F16, 64), (BF16, BF16, 128), (F16, F16, 64)])
+@pytest.mark.parametrize("k_scale", [8.0, 0.0])
+def test_large_and_equal_scores(ctx, dev, dtype, kv, hd, k_scale):
+    # scores up to some hundred: the running maximum moves often and far; and all equal: every weight is the same
+    c = Case(ctx, dev, lens=[700, 90], drafts=[40, 90], hq=4, hkv=2, hd=hd, dtype=dtype, kv=kv, k_scale=k_scale, scale=0.5, seed=41)
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv,hd", [(F32, F16, 64), (BF16, BF16, 128), (F16, F16, 64)])
+def test_many_sequences(ctx, dev, dtype, kv, hd):
+    rng = np.random.default_rng(3)
+    n = 300  # more than one pass of the walk's sum takes
+    drafts = rng.integers(1, 4, n)
+    c = Case(ctx, dev, lens=drafts + rng.integers(0, 200, n), drafts=drafts, hq=2, hkv=1, hd=hd, dtype=dtype, kv=kv, seed=43)
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv", [(F32, F16), (BF16, BF16)])
+def test_bad_sequences_are_reported_and_left_alone(ctx, dev, dtype, kv):
+    c = Case(ctx, dev, lens=[50, 60, 70], drafts=[3, 4, 5], hq=4, hkv=2, hd=64, dtype=dtype, kv=kv, seed=51)
+    c.run()
+    want = dev.get(c.d["out"])
+    for change in ("slot", "length", "rows"):
+        d = c.upload()
+        if change == "slot":
+            d["slots"][1] = 99
+        elif change == "length":
+            d["lens"][1] = 3  # fewer positions than drafted rows
+        else:
+            d["starts"][3] = 13  # one row more than the call has
+        c.call()
+        with pytest.raises(L.LokalCudaError) as e:
+            ctx.stream_sync()
+        assert e.value.status == capi.ERR_PAGE_RANGE
+        got, lost = dev.get(d["out"]), slice(3, 7) if change != "rows" else slice(7, 12)
+        assert (got[lost] == c.fill).all()
+        keep = np.ones(12, bool)
+        keep[lost] = False
+        assert np.allclose(got[keep], want[keep], rtol=2e-2, atol=2e-2) and (got[keep] != c.fill).any()
+    # a page that is not there: reported, nothing outside the pool is read
+    d = c.upload()
+    d["table"][1, 1] = -1
+    d["table"][2, 0] = 1 << 30
+    c.call()
+    with pytest.raises(L.LokalCudaError) as e:
+        ctx.stream_sync()
+    assert e.value.status == capi.ERR_PAGE_RANGE
+    assert np.allclose(dev.get(d["out"])[:3], want[:3], rtol=2e-2, atol=2e-2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv", [(F32, F16), (BF16, BF16)])
+def test_captured_and_on_two_streams(ctx, dev, dtype, kv):
+    a = Case(ctx, dev, lens=[500, 1200], drafts=[8, 30], hq=4, hkv=2, hd=64, dtype=dtype, kv=kv, seed=61)
+    b = Case(ctx, dev, lens=[90], drafts=[3], hq=4, hkv=2, hd=64, dtype=dtype, kv=kv, seed=62)
+    first, second = a.run(), b.run()
+    s, t = ctx.stream_create(), ctx.stream_create()
+    a.torch.cuda.synchronize()
+    ctx.graph_begin(s)
+    a.call(stream=s)
+    graph = ctx.graph_end(s)
+    for _ in range(5):
+        a.d["out"].fill_(0.0)
+        b.d["out"].fill_(0.0)
+        a.torch.cuda.synchronize()
+        ctx.graph_launch(graph, s)
+        b.call(stream=t)
+        ctx.stream_sync(s)
+        ctx.stream_sync(t)
+        assert np.array_equal(dev.get(a.d["out"])[:, :256], first[:, :256]) and np.array_equal(dev.get(b.d["out"])[:, :256], second[:, :256])
+    # the lengths are read when the graph runs: a shorter sequence, same graph
+    a.lens[1] = 700
+    a.d["lens"].copy_(dev.put(np.array([500, 700, 0], np.int32)))
+    a.torch.cuda.synchronize()
+    ctx.graph_launch(graph, s)
+    ctx.stream_sync(s)
+    a.fill = 0.0
+    a.check(dev.get(a.d["out"]))
+    ctx.graph_destroy(graph)
+    ctx.stream_destroy(s)
+    ctx.stream_destroy(t)
+
+
+@pytest.mark.gpu
+def test_refusals(ctx, dev):
+    c = Case(ctx, dev, lens=[50], drafts=[3], hq=4, hkv=2, hd=64, dtype=BF16, kv=BF16, seed=71)
+    d = c.upload()
+    for over, status in [(dict(k_store=2), capi.ERR_BAD_ARG), (dict(dtype=L.Q8_0), capi.ERR_UNSUPPORTED), (dict(kv_dtype=L.Q8_0), capi.ERR_UNSUPPORTED),
+                         (dict(n_q_heads=5), capi.ERR_BAD_ARG), (dict(n_kv_heads=0), capi.ERR_BAD_ARG), (dict(head_dim=0), capi.ERR_BAD_ARG),
+                         (dict(head_dim=257, n_kv_heads=1, n_q_heads=1), capi.ERR_UNSUPPORTED), (dict(n_kv_heads=4), capi.ERR_BAD_ARG),
+                         (dict(kv_dtype=F32), capi.ERR_BAD_ARG), (dict(mask_words=0), capi.ERR_BAD_ARG), (dict(q_row_stride=255), capi.ERR_BAD_ARG),
+                         (dict(out_row_stride=1), capi.ERR_BAD_ARG), (dict(workspace=None), capi.ERR_BAD_ARG),
+                         (dict(workspace_bytes=d["bytes"] - 1), capi.ERR_BAD_ARG), (dict(workspace=d["work"].data_ptr() + 8), capi.ERR_MISALIGNED),
+                         (dict(q_start=None), capi.ERR_BAD_ARG), (dict(mask=d["mask"].data_ptr() + 4), capi.ERR_MISALIGNED)]:
+        with pytest.raises(L.LokalCudaError) as e:
+            c.call(**over)
+        assert e.value.status == status, over
+    for x in ("q", "out"):
+        with pytest.raises(L.LokalCudaError) as e:
+            ctx.tree_attn(d["pool"], d["q"].data_ptr() + (x == "q"), d["out"].data_ptr() + (x == "out"), k_store=0, v_store=1, q_start=d["starts"], n_seqs=1,
+                          rows=3, n_q_heads=4, n_kv_heads=2, head_dim=64, scale=1.0, dtype=BF16, kv_dtype=BF16, workspace=d["work"], workspace_bytes=d["bytes"])
+        assert e.value.status == capi.ERR_MISALIGNED
+    c.call(n_seqs=0)
+    c.call(rows=0)
+    ctx.stream_sync()
+    assert (dev.get(d["out"]) == c.fill).all(), "a refused or empty call writes nothing"
+    assert ctx.tree_attn_workspace(rows=3, n_q_heads=4, n_kv_heads=2, head_dim=300) == 0
+
+
+# ---- the plan ----
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("chain", [False, True])
+def test_plan_follows_the_parents(ctx, dev, chain):
+    import torch
+    c = Case(ctx, dev, lens=[9, 300, 131, 70], drafts=[9, 200, 0, 65], hq=1, hkv=1, hd=8, seed=81, extra_rows=3)
+    rng = np.random.default_rng(1)
+    parents = [np.arange(n) - 1 if chain else random_parents(rng, int(n)) for n in c.drafts]
+    d = c.upload()
+    words = 4
+    mask = torch.full((c.rows, words), -1, dtype=torch.int64, device="cuda")
+    pos = torch.full((c.rows,), -9, dtype=torch.int32, device="cuda")
+    rows = torch.full((c.rows,), -9, dtype=torch.int32, device="cuda")
+    up = None if chain else dev.put(np.concatenate([*parents, np.zeros(3)]).astype(np.int32))
+    ctx.tree_plan(d["pool"], q_start=d["starts"], slots=d["slots"], n_seqs=4, rows=c.rows, parents=up, mask=mask, mask_words=words, positions=pos,
+                  cache_rows=rows)
+    ctx.stream_sync()
+    mask, pos, rows = mask.cpu().numpy().view(np.uint64), pos.cpu().numpy(), rows.cpu().numpy()
+    for i, p in enumerate(parents):
+        r0, n, base = int(c.starts[i]), len(p), int(c.lens[i] - c.drafts[i])
+        depth = np.zeros(n, int)
+        for j, a in enumerate(p):
+            depth[j] = depth[a] + 1 if a >= 0 else 0
+        assert np.array_equal(mask[r0:r0 + n], mask_of(p, words))
+        assert np.array_equal(pos[r0:r0 + n], base + depth)
+        assert np.array_equal(rows[r0:r0 + n], c.cache_row(i, base + np.arange(n)))
+    assert (mask[-3:] == np.uint64(2 ** 64 - 1)).all() and (pos[-3:] == -9).all() and (rows[-3:] == -9).all()
+
+
+@pytest.mark.gpu
+def test_plan_reports_bad_parents_and_narrow_masks(ctx, dev):
+    import torch
+    c = Case(ctx, dev, lens=[80], drafts=[70], hq=1, hkv=1, hd=8, seed=82)
+    d = c.upload()
+    mask = torch.zeros((70, 2), dtype=torch.int64, device="cuda")
+    parents = random_parents(np.random.default_rng(2), 70)
+    for j, bad in ((5, 5), (6, 40), (7, -2), (0, 3)):
+        p = parents.copy()
+        p[j] = bad
+        ctx.tree_plan(d["pool"], q_start=d["starts"], n_seqs=1, rows=70, parents=dev.put(p), mask=mask, mask_words=2)
+        with pytest.raises(L.LokalCudaError) as e:
+            ctx.stream_sync()
+        assert e.value.status == capi.ERR_PAGE_RANGE
+        p[j] = -1
+        assert np.array_equal(mask.cpu().numpy().view(np.uint64), mask_of(p, 2))
+    ctx.tree_plan(d["pool"], q_start=d["starts"], n_seqs=1, rows=70, parents=dev.put(parents), mask=mask, mask_words=1)
+    with pytest.raises(L.LokalCudaError) as e:
+        ctx.stream_sync()
+    assert e.value.status == capi.ERR_PAGE_RANGE
+    for kw in (dict(mask_words=0), dict(q_start=None)):
+        with pytest.raises(L.LokalCudaError) as e:
+            ctx.tree_plan(d["pool"], **{**dict(q_start=d["starts"], n_seqs=1, rows=70, mask=mask, mask_words=1), **kw})
+        assert e.value.status == capi.ERR_BAD_ARG
+
+
+# ---- all of it together ----
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv", [(BF16, BF16), (F32, F16)])
+def test_draft_verify_accept_steps(ctx, dev, dtype, kv):
+    """Two prompts, one forked, then steps of: grow, plan, rotate K into the cache, stage V, attend, accept a path, compact. The
+    attention of every step agrees with a plain one over the rows that each sequence should hold by then."""
+    import torch
+    cfg = synth.LayerConfig("steps", dtype, 64, 64, 64, 4, 2, 64, 100, 1e4, 1e-6, 1, seed=90)
+    hq, hkv, hd, page, n_pages, n_slots = 4, 2, 64, 16, 60, 4
+    width = hkv * hd
+    rng = np.random.default_rng(17)
+    put = dev.put
+    ints = lambda a: put(np.asarray(a, np.int32))
+    kstore, vstore = dev.empty((n_pages * page, width), kv, fill=3.0), dev.empty((n_pages * page, width), kv, fill=3.0)
+    table, lens, refs = (torch.zeros(s, dtype=torch.int32, device="cuda") for s in ((n_slots, 20), (n_slots,), (n_pages,)))
+    pool = L.KvPool(ctx, page_rows=page, n_pages=n_pages, n_slots=n_slots, max_pages=20, table=table, lens=lens, refs=refs, stores=[kstore, vstore],
+                    row_bytes=width * kstore.element_size())
+    pool.reset()
+    held = {}  # slot -> list of (k row, v row) as the cache should hold them
+
+    def stage(slots, n_rows, parents):
+        """Grows, plans and stages; returns what the attention call needs."""
+        starts = np.concatenate([[0], np.cumsum(n_rows)])
+        rows, words = int(starts[-1]), -(-max(n_rows) // 64)
+        dslots, dstarts = ints(slots), ints(starts)
+        pool.reserve(dslots, ints([len(held[s]) + n for s, n in zip(slots, n_rows)]), n=len(slots))
+        mask = torch.zeros((rows, words), dtype=torch.int64, device="cuda") if parents is not None else None
+        pos, crow = torch.zeros(rows, dtype=torch.int32, device="cuda"), torch.zeros(rows, dtype=torch.int32, device="cuda")
+        up = None if parents is None else ints(np.concatenate(parents))
+        ctx.tree_plan(pool, slots=dslots, q_start=dstarts, n_seqs=len(slots), rows=rows, parents=up, mask=mask, mask_words=words if mask is not None else 0,
+                      positions=pos, cache_rows=crow)
+        q, k, v = (synth.round_to(rng.standard_normal((rows, w), dtype=np.float32), dtype) for w in (hq * hd, width, width))
+        dq, dk, dv = put(q, dtype), put(k, dtype), put(v, dtype)
+        rope = torch.zeros((rows, hd), dtype=torch.float32, device="cuda")
+        ctx.rope_table(rope, theta=cfg.theta, rot_dim=hd, rows=rows, positions=pos)
+        p = ctx.qk_rope_params(q=dq, k=dk, k_out=dk, cos_sin=rope, rows=rows, n_q_heads=hq, n_kv_heads=hkv, head_dim=hd, q_dtype=dtype, k_dtype=dtype, w_dtype=F32)
+        ctx.qk_rope(p)
+        for src, dst in ((dk, kstore), (dv, vstore)):
+            ctx.kv_stage(src, dst, src_dtype=dtype, dst_dtype=kv, rows=rows, width=width, dst_rows=crow)
+        ctx.stream_sync()
+        kk, vv = synth.round_to(dev.get(dk), kv), synth.round_to(v, kv)
+        return starts, mask, dq, kk, vv, dslots, dstarts, rows, words
+
+    def attend_and_check(slots, n_rows, made):
+        starts, mask, dq, kk, vv, dslots, dstarts, rows, words = made
+        out = dev.empty((rows, hq * hd), dtype, fill=0.0)
+        nbytes = ctx.tree_attn_workspace(rows=rows, n_q_heads=hq, n_kv_heads=hkv, head_dim=hd)
+        work = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+        ctx.tree_attn(pool, dq, out, k_store=0, v_store=1, slots=dslots, q_start=dstarts, n_seqs=len(slots), rows=rows, mask=mask,
+                      mask_words=words if mask is not None else 0, n_q_heads=hq, n_kv_heads=hkv, head_dim=hd, scale=hd ** -0.5, dtype=dtype, kv_dtype=kv,
+                      workspace=work, workspace_bytes=nbytes)
+        ctx.stream_sync()
+        got, q = dev.get(out), dev.get(dq)
+        bits_ = None if mask is None else mask.cpu().numpy().view(np.uint64)
+        for i, s in enumerate(slots):
+            r0, n = int(starts[i]), n_rows[i]
+            ks = np.concatenate([np.array([a for a, _ in held[s]], np.float32).reshape(-1, width), kk[r0:r0 + n]])
+            vs = np.concatenate([np.array([b for _, b in held[s]], np.float32).reshape(-1, width), vv[r0:r0 + n]])
+            see = visible(n, len(held[s]), None if bits_ is None else bits_[r0:r0 + n])
+            for h in range(hq):
+                kc, qc = slice(h // 2 * hd, (h // 2 + 1) * hd), slice(h * hd, (h + 1) * hd)
+                o, size, terms = attention(q[r0:r0 + n, qc], ks[:, kc], vs[:, kc], see, np.float32(hd ** -0.5))
+                assert (np.abs(got[r0:r0 + n, qc] - o) <= tolerance(o, size, terms, len(ks), hd, dtype, dtype == kv)).all()
+
+    # prompts, as chains
+    held[0], held[1] = [], []
+    made = stage([0, 1], [37, 90], None)
+    attend_and_check([0, 1], [37, 90], made)
+    for s, r0, n in ((0, 0, 37), (1, 37, 90)):
+        held[s] = [(made[3][r0 + j], made[4][r0 + j]) for j in range(n)]
+    pool.fork(ints([1]), ints([2]), n=1)
+    held[2] = list(held[1])
+    for step in range(4):
+        slots = [0, 1, 2]
+        n_rows = [int(x) for x in rng.integers(1, 40, 3)]
+        parents = [random_parents(rng, n) for n in n_rows]
+        made = stage(slots, n_rows, parents)
+        attend_and_check(slots, n_rows, made)
+        # one path from a child of the last committed row down
+        acc, counts = np.zeros((3, 8), np.int32), []
+        for i in range(3):
+            path, at = [], -1
+            while len(path) < 8:
+                children = [j for j in range(n_rows[i]) if parents[i][j] == at]
+                if not children:
+                    break
+                at = int(rng.choice(children))
+                path.append(at)
+            acc[i, :len(path)] = path
+            counts.append(len(path))
+            held[slots[i]] += [(made[3][made[0][i] + j], made[4][made[0][i] + j]) for j in path]
+        pool.accept(made[5], made[6], ints(acc.reshape(-1)), ints(counts), n_seqs=3, max_accept=8)
+        if step == 1:
+            pool.truncate(ints([0]), n=1)
+            held[0] = []
+        if step % 2:
+            pool.compact()
+        ctx.stream_sync()
+        assert list(lens.cpu().numpy()[:3]) == [len(held[s]) for s in slots]
+    pool.close()
