@@ -254,7 +254,7 @@ int launch_any_q(lokal_cuda_ctx* ctx, cudaStream_t s, const TreeArgs& a, int kv_
     }
 }
 
-size_t part_bytes(size_t shares, size_t rows, size_t head_dim) { return shares * 2 * rows * (head_dim + 2) * sizeof(float); }
+size_t any_rows(const lokal_cuda_ctx* ctx, unsigned head_dim) { return static_cast<size_t>(ctx->sm_count) * any_ctas(head_dim) * 2 * kAnyRows; }
 
 // ---- mask, positions and cache rows of drafted trees ----
 struct PlanArgs {
@@ -351,8 +351,8 @@ int lokal_cuda_tree_plan(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const lokal_k
 
 size_t lokal_cuda_tree_attn_workspace(const lokal_cuda_ctx* ctx, size_t rows, uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t head_dim) {
     if (!ctx || rows == 0 || n_q_heads == 0 || n_kv_heads == 0 || head_dim == 0 || head_dim > 256) return 0;
-    const size_t sms = static_cast<size_t>(ctx->sm_count);
-    return lokal::part_bytes(sms * lokal::any_ctas(head_dim), lokal::kAnyRows, head_dim);
+    const size_t any = lokal::any_rows(ctx, head_dim), tc = head_dim == 64 || head_dim == 128 ? lokal::tree_tc_rows(ctx) : 0;
+    return (any > tc ? any : tc) * (head_dim + 2) * sizeof(float);
 }
 
 int lokal_cuda_tree_attn(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const lokal_kv_pool* pool, uint32_t k_store, uint32_t v_store,
@@ -402,10 +402,12 @@ int lokal_cuda_tree_attn(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const lokal_k
     a.group = n_q_heads / n_kv_heads;
     a.head_dim = head_dim;
     a.scale_log2 = scale * 1.4426950408889634f;
-    const size_t shares = static_cast<size_t>(ctx->sm_count) * lokal::any_ctas(head_dim);
-    a.part_ml = static_cast<float2*>(workspace);
-    a.part_o = reinterpret_cast<float*>(a.part_ml + shares * 2 * lokal::kAnyRows);
+    a.wait_limit = static_cast<unsigned>(lokal::tune_env("LOKAL_CUDA_WAIT_LIMIT", lokal::kWaitLimit));
     cudaStream_t st = static_cast<cudaStream_t>(s);
+    const bool tc = lokal::tree_tc_takes(a, dtype, kv_dtype);
+    a.part_ml = static_cast<float2*>(workspace);
+    a.part_o = reinterpret_cast<float*>(a.part_ml + (tc ? lokal::tree_tc_rows(ctx) : lokal::any_rows(ctx, head_dim)));
+    if (tc) return lokal::launch_tree_tc(ctx, st, a, dtype);
     switch (dtype) {
         case LOKAL_F32: return lokal::launch_any_q<float>(ctx, st, a, kv_dtype);
         case LOKAL_F16: return lokal::launch_any_q<__half>(ctx, st, a, kv_dtype);

@@ -249,6 +249,11 @@ inline cudaError_t launch_staged(void (*kernel)(KArgs...), dim3 grid, dim3 block
     return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
 }
 
+// The tensor-core kernel (treeattn_tc.cu): whether it takes a call, the rows of pieces it may leave, and its launch.
+bool tree_tc_takes(const TreeArgs& a, int dtype, int kv_dtype);
+size_t tree_tc_rows(const lokal_cuda_ctx* ctx);
+int launch_tree_tc(lokal_cuda_ctx* ctx, cudaStream_t s, const TreeArgs& a, int dtype);
+
 // Joins the pieces of blocks that several CTAs share. CTA c stands at the border between shares c and c + 1; the CTAs at
 // the borders inside one block divide its rows among them. One warp per row.
 template <typename T, int R, int KT>
