@@ -59,14 +59,14 @@ __global__ void __launch_bounds__(kAnyThreads) tree_attn_any_kernel(const TreeAr
     unsigned long long* sh = row_at + kAnyKeys;
     const unsigned tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     const unsigned shares = gridDim.x;
-    const TreePlace place = tree_locate<kAnyRows, kAnyKeys, kAnyThreads>(a, sh, blockIdx.x == 0, [&](unsigned long long total) {
-        const unsigned g = total < shares ? static_cast<unsigned>(total) : shares;
-        return blockIdx.x < g ? tree_share(total, blockIdx.x, g) : total;
+    const TreePlace place = tree_locate<kAnyKeys, kAnyThreads>(a, sh, blockIdx.x == 0, [&](unsigned total) {
+        const TreeShares s(total, shares);
+        return blockIdx.x < s.g ? s.first(blockIdx.x) : total;
     });
     if (place.seq >= a.n_seqs) return;
-    const unsigned g = place.total < shares ? static_cast<unsigned>(place.total) : shares;
-    TreeWalk<kAnyRows, kAnyKeys> walk;
-    walk.start(a, place, tree_share(place.total, blockIdx.x, g), tree_share(place.total, blockIdx.x + 1, g));
+    const TreeShares share(place.total, shares);
+    TreeWalk<kAnyKeys> walk;
+    walk.start(a, place, share.first(blockIdx.x), share.first(blockIdx.x + 1));
     TreeUnit u;
     const unsigned hd = a.head_dim;
     while (walk.next(a, u)) {
@@ -405,6 +405,7 @@ int lokal_cuda_tree_attn(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const lokal_k
     a.wait_limit = static_cast<unsigned>(lokal::tune_env("LOKAL_CUDA_WAIT_LIMIT", lokal::kWaitLimit));
     cudaStream_t st = static_cast<cudaStream_t>(s);
     const bool tc = lokal::tree_tc_takes(a, dtype, kv_dtype);
+    a.block_rows = tc ? lokal::tree_tc_block(a) : lokal::kAnyRows;
     a.part_ml = static_cast<float2*>(workspace);
     a.part_o = reinterpret_cast<float*>(a.part_ml + (tc ? lokal::tree_tc_rows(ctx) : lokal::any_rows(ctx, head_dim)));
     if (tc) return lokal::launch_tree_tc(ctx, st, a, dtype);

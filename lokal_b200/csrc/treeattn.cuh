@@ -1,7 +1,7 @@
 // What the two attention kernels (treeattn.cu: any type and shape; treeattn_tc.cu: 16-bit rows on the tensor cores) and
 // the launch that joins their pieces share: the arguments, the walk over the work, the visibility of drafted rows.
 //
-// The work of a call is a list of tiles: for every sequence, key head and block of R query rows (a row is one drafted
+// The work of a call is a list of tiles: for every sequence, key head and block of up to R query rows (a row is one drafted
 // row and one of the query heads that share the key head), the sequence's keys in tiles of KT. The lengths are on the
 // device, so the list is too: every CTA sums it up for itself and takes an equal, contiguous share of it, whatever the
 // lengths. A block whose tiles fall to several CTAs is left by each as a piece (sums that are not yet divided, with
@@ -29,6 +29,7 @@ struct TreeArgs {
     unsigned long long q_stride, out_stride, row_bytes;
     unsigned n_seqs, rows, mask_words, n_q_heads, n_kv_heads, group, head_dim;
     unsigned page_rows, page_shift, n_pages, n_slots, max_pages;
+    unsigned block_rows;  // query rows of a block: at most R
     unsigned wait_limit;
     float scale_log2;  // scale * log2(e): the exponentials are powers of two
 };
@@ -59,46 +60,55 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, unsigned i, bool 
     return q;
 }
 
-template <int R, int KT>
+template <int KT>
 __device__ __forceinline__ unsigned long long tree_tiles(const TreeArgs& a, const TreeSeq& q) {
-    const unsigned long long blocks = (static_cast<unsigned long long>(q.n) * a.group + R - 1) / R;
+    const unsigned long long blocks = (q.n * a.group + a.block_rows - 1) / a.block_rows;  // rows * heads fit 31 bits
     return blocks * a.n_kv_heads * ((static_cast<unsigned>(q.len) + KT - 1) / KT);
 }
 
-// First tile of share c of g over `total` tiles.
-__device__ __forceinline__ unsigned long long tree_share(unsigned long long total, unsigned c, unsigned g) {
-    return total * c / g;
-}
+// The tiles of a call dealt to g CTAs: share c is [first(c), first(c + 1)), the first `extra` shares one tile longer.
+struct TreeShares {
+    unsigned g, len, extra;
+    __device__ TreeShares(unsigned total, unsigned most) {
+        g = total < most ? total : most;
+        len = g ? total / g : 0u;
+        extra = g ? total - len * g : 0u;
+    }
+    __device__ unsigned first(unsigned c) const { return c * len + min(c, extra); }
+    __device__ unsigned owner(unsigned tile) const {
+        const unsigned longer = extra * (len + 1);
+        return tile < longer ? tile / (len + 1) : extra + (tile - longer) / len;
+    }
+};
 
 struct TreePlace {
-    unsigned long long total;  // tiles of the call
-    unsigned long long base;   // tiles before sequence `seq`
-    unsigned seq;
+    unsigned total;  // tiles of the call
+    unsigned base;   // tiles before sequence `seq`
+    unsigned seq;    // n_seqs: nothing to do
 };
 
 // Whole CTA (NT threads): the sum of all tiles, then, for the tile number that `pick` makes of it, the sequence that
-// holds the tile. `sh` is 2 * (NT / 32) + 4 words of shared memory. Sequences are summed NT at a time, so any number of them.
-template <int R, int KT, int NT, typename Pick>
+// holds the tile. `sh` is 2 * (NT / 32) + 4 words of shared memory. Sequences are summed NT at a time, so any number of
+// them; up to NT take one trip to memory. More than 2^32 - 1 tiles are refused.
+template <int KT, int NT, typename Pick>
 __device__ TreePlace tree_locate(const TreeArgs& a, unsigned long long* sh, bool report, Pick pick) {
     constexpr unsigned kWarps = NT / 32;
     const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    unsigned long long sum = 0;
-    for (unsigned i = threadIdx.x; i < a.n_seqs; i += NT) sum += tree_tiles<R, KT>(a, tree_seq(a, i, report));
+    TreePlace p{0u, 0u, a.n_seqs};
+    unsigned long long total = 0;
+    if (a.n_seqs > NT) {
+        unsigned long long sum = 0;
+        for (unsigned i = threadIdx.x; i < a.n_seqs; i += NT) sum += tree_tiles<KT>(a, tree_seq(a, i, report));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) sh[warp] = sum;
-    __syncthreads();
-    TreePlace p{0, 0, 0};
-    for (unsigned w = 0; w < kWarps; w++) p.total += sh[w];
-    const unsigned long long at = pick(p.total);
-    if (at >= p.total) {
-        p.seq = a.n_seqs;
-        return p;
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) sh[warp] = sum;
+        __syncthreads();
+        for (unsigned w = 0; w < kWarps; w++) total += sh[w];
     }
     unsigned long long before = 0;
     for (unsigned base = 0; base < a.n_seqs; base += NT) {
         const unsigned i = base + threadIdx.x;
-        const unsigned long long mine = i < a.n_seqs ? tree_tiles<R, KT>(a, tree_seq(a, i, false)) : 0;
+        const unsigned long long mine = i < a.n_seqs ? tree_tiles<KT>(a, tree_seq(a, i, report && a.n_seqs <= NT)) : 0;
         unsigned long long s = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -114,21 +124,29 @@ __device__ TreePlace tree_locate(const TreeArgs& a, unsigned long long* sh, bool
             if (w < warp) off += t;
             all += t;
         }
-        const unsigned long long from = off + s - mine;
-        if (at >= from && at < off + s) {
-            sh[kWarps] = from;
+        if (a.n_seqs <= NT) total = all;
+        if (total > 0xffffffffull) {
+            if (report && threadIdx.x == 0) atomicOr(a.err_word, kErrPageRange);
+            return p;
+        }
+        p.total = static_cast<unsigned>(total);
+        const unsigned at = pick(p.total);
+        if (at >= p.total) return p;
+        if (at >= off + s - mine && at < off + s) {
+            sh[kWarps] = off + s - mine;
             sh[kWarps + 1] = i;
         }
-        if (at < before + all) break;  // the same for every thread
         before += all;
+        if (at < before) break;  // the same for every thread
     }
     __syncthreads();
-    p.base = sh[kWarps];
+    if (p.total == 0) return p;
+    p.base = static_cast<unsigned>(sh[kWarps]);
     p.seq = static_cast<unsigned>(sh[kWarps + 1]);
     return p;
 }
 
-// A block of R rows of one sequence and key head, and the CTA's run of its key tiles.
+// A block of rows of one sequence and key head, and the CTA's run of its key tiles.
 struct TreeUnit {
     TreeSeq seq;
     unsigned kv_head, block;
@@ -138,13 +156,11 @@ struct TreeUnit {
 };
 
 // Steps through the tiles [at, hi) of a CTA. Every role of a CTA walks for itself.
-template <int R, int KT>
+template <int KT>
 struct TreeWalk {
-    unsigned long long at, hi, lo, base;
-    unsigned seq;
+    unsigned at, hi, lo, base, cur_tiles, seq;
     TreeSeq cur;
-    unsigned long long cur_tiles;
-    __device__ void start(const TreeArgs& a, const TreePlace& p, unsigned long long from, unsigned long long to) {
+    __device__ void start(const TreeArgs& a, const TreePlace& p, unsigned from, unsigned to) {
         lo = at = from;
         hi = to;
         base = p.base;
@@ -155,26 +171,25 @@ struct TreeWalk {
     }
     __device__ void load(const TreeArgs& a) {
         cur = tree_seq(a, seq, false);
-        cur_tiles = tree_tiles<R, KT>(a, cur);
+        cur_tiles = static_cast<unsigned>(tree_tiles<KT>(a, cur));
     }
     __device__ bool next(const TreeArgs& a, TreeUnit& u) {
         if (at >= hi) return false;
-        while (at >= base + cur_tiles) {
+        while (at - base >= cur_tiles) {
             base += cur_tiles;
             seq++;
             if (seq >= a.n_seqs) return false;  // only if the arrays changed under the call
             load(a);
         }
-        const unsigned long long off = at - base;
+        const unsigned off = at - base;
         const unsigned kt = (static_cast<unsigned>(cur.len) + KT - 1) / KT;
-        const unsigned blocks = static_cast<unsigned>((static_cast<unsigned long long>(cur.n) * a.group + R - 1) / R);
-        const unsigned long long unit = off / kt;
+        const unsigned blocks = (cur.n * a.group + a.block_rows - 1) / a.block_rows;
+        const unsigned unit = off / kt;
         u.seq = cur;
-        u.kv_head = static_cast<unsigned>(unit / blocks);
-        u.block = static_cast<unsigned>(unit % blocks);
-        u.k0 = static_cast<unsigned>(off % kt);
-        const unsigned long long left = hi - at;
-        u.k1 = left < kt - u.k0 ? u.k0 + static_cast<unsigned>(left) : kt;
+        u.kv_head = unit / blocks;
+        u.block = unit - u.kv_head * blocks;
+        u.k0 = off - unit * kt;
+        u.k1 = min(kt, u.k0 + (hi - at));
         u.whole = u.k0 == 0 && u.k1 == kt;
         u.piece = lo >= base + unit * kt ? 0u : 1u;
         at += u.k1 - u.k0;
@@ -249,49 +264,56 @@ inline cudaError_t launch_staged(void (*kernel)(KArgs...), dim3 grid, dim3 block
     return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
 }
 
-// The tensor-core kernel (treeattn_tc.cu): whether it takes a call, the rows of pieces it may leave, and its launch.
+// The tensor-core kernel (treeattn_tc.cu): whether it takes a call, the rows of its blocks and of the pieces it may leave,
+// and its launch.
 bool tree_tc_takes(const TreeArgs& a, int dtype, int kv_dtype);
+unsigned tree_tc_block(const TreeArgs& a);
 size_t tree_tc_rows(const lokal_cuda_ctx* ctx);
 int launch_tree_tc(lokal_cuda_ctx* ctx, cudaStream_t s, const TreeArgs& a, int dtype);
 
 // Joins the pieces of blocks that several CTAs share. CTA c stands at the border between shares c and c + 1; the CTAs at
-// the borders inside one block divide its rows among them. One warp per row.
+// the borders inside one block divide its rows among them. A warp takes a row, or, where a CTA has fewer rows than warps,
+// a part of a row's pieces (a single block may be in as many pieces as there are shares); 32 pieces are weighed at once,
+// a lane each, and eight loads are in flight.
 template <typename T, int R, int KT>
 __global__ void __launch_bounds__(256) tree_join_kernel(const TreeArgs a, unsigned shares) {
     pdl_sync();
     __shared__ unsigned long long sh[2 * 8 + 4];
+    __shared__ float part[8][256];
+    __shared__ float part_l[8];
     const unsigned c = blockIdx.x + 1;
-    const TreePlace p = tree_locate<R, KT, 256>(a, sh, false, [&](unsigned long long total) {
-        const unsigned g = total < shares ? static_cast<unsigned>(total) : shares;
-        return c < g ? tree_share(total, c, g) : total;
+    const TreePlace p = tree_locate<KT, 256>(a, sh, false, [&](unsigned total) {
+        const TreeShares s(total, shares);
+        return c < s.g ? s.first(c) : total;
     });
     if (p.seq >= a.n_seqs) return;
-    const unsigned g = p.total < shares ? static_cast<unsigned>(p.total) : shares;
-    const unsigned long long border = tree_share(p.total, c, g);
+    const TreeShares s(p.total, shares);
+    const unsigned border = s.first(c);
     const TreeSeq q = tree_seq(a, p.seq, false);
     const unsigned kt = (static_cast<unsigned>(q.len) + KT - 1) / KT;
-    const unsigned rows_all = q.n * a.group, blocks = (rows_all + R - 1) / R;
-    const unsigned long long unit = (border - p.base) / kt;
-    const unsigned long long t0 = p.base + unit * kt, t1 = t0 + kt;
+    const unsigned rows_all = q.n * a.group, blocks = (rows_all + a.block_rows - 1) / a.block_rows;
+    const unsigned unit = (border - p.base) / kt;
+    const unsigned t0 = p.base + unit * kt, t1 = t0 + kt;
     if (border == t0) return;
-    // borders inside (t0, t1): floor(total * x / g) > t0 and < t1
-    const unsigned first = static_cast<unsigned>(((t0 + 1) * g + p.total - 1) / p.total);
-    const unsigned last = static_cast<unsigned>((t1 * g + p.total - 1) / p.total) - 1u < g - 1u
-                              ? static_cast<unsigned>((t1 * g + p.total - 1) / p.total) - 1u : g - 1u;
-    const unsigned n_borders = last - first + 1;
-    const unsigned kv_head = static_cast<unsigned>(unit / blocks), block = static_cast<unsigned>(unit % blocks);
-    const unsigned m_rows = min(static_cast<unsigned>(R), rows_all - block * R);
+    const unsigned first = s.owner(t0) + 1, last = s.owner(t1 - 1);  // borders inside the block
+    const unsigned n_borders = last - first + 1, n_pieces = n_borders + 1;
+    const unsigned kv_head = unit / blocks, block = unit - kv_head * blocks;
+    const unsigned m_rows = min(a.block_rows, rows_all - block * a.block_rows);
     const unsigned r0 = m_rows * (c - first) / n_borders, r1 = m_rows * (c - first + 1) / n_borders;
-    const unsigned lane = threadIdx.x & 31u;
-    const bool first_is_0 = tree_share(p.total, first - 1, g) >= t0;
-    for (unsigned r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
-        const unsigned flat = block * R + r, node = flat / a.group, head = kv_head * a.group + flat % a.group;
+    const unsigned lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const bool first_is_0 = s.first(first - 1) >= t0;
+    const unsigned rows = r1 - r0, parts = rows <= 1 ? 8u : rows <= 2 ? 4u : rows <= 4 ? 2u : 1u, step = 8u / parts;
+    const unsigned x0 = n_pieces * (warp % parts) / parts, x1 = n_pieces * (warp % parts + 1) / parts;
+    for (unsigned rr = r0; rr < r1; rr += step) {  // the same number of rounds for every warp
+        const unsigned r = rr + warp / parts;
+        const bool in = r < r1;
         // piece x (0 ..) is left by share first - 1 + x; only the first of them may be a CTA's second block
         auto slot_of = [&](unsigned x) {
             return (static_cast<size_t>(first - 1 + x) * 2 + (x == 0 && !first_is_0 ? 1 : 0)) * R + r;
         };
         float m = -INFINITY;
-        for (unsigned x = lane; x <= n_borders; x += 32) m = fmaxf(m, a.part_ml[slot_of(x)].x);
+        if (in)
+            for (unsigned x = lane; x < n_pieces; x += 32) m = fmaxf(m, a.part_ml[slot_of(x)].x);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         const float ref = m == -INFINITY ? 0.0f : m;
@@ -299,17 +321,41 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeArgs a, unsign
 #pragma unroll
         for (int j = 0; j < 8; j++) acc[j] = 0.0f;
         float l = 0.0f;
-        for (unsigned x = 0; x <= n_borders; x++) {
-            const size_t s = slot_of(x);
-            const float2 ml = a.part_ml[s];
-            if (ml.y == 0.0f) continue;  // nothing of this piece was visible
-            const float w = exp2f(ml.x - ref);
-            l = fmaf(ml.y, w, l);
-            const float* o = a.part_o + s * a.head_dim;
+        for (unsigned x = in ? x0 : x1; x < x1; x += 32) {
+            float w = 0.0f;  // stays 0 where nothing of a piece was visible
+            if (x + lane < x1) {
+                const float2 ml = a.part_ml[slot_of(x + lane)];
+                if (ml.y != 0.0f) {
+                    w = exp2f(ml.x - ref);
+                    l = fmaf(ml.y, w, l);
+                }
+            }
+            const unsigned n = min(32u, x1 - x);
+#pragma unroll 8
+            for (unsigned i = 0; i < n; i++) {
+                const float wi = __shfl_sync(0xffffffffu, w, i);
+                const float* o = a.part_o + slot_of(x + i) * a.head_dim;
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (j * 32 + lane < a.head_dim) acc[j] = fmaf(o[j * 32 + lane], w, acc[j]);
+                for (int j = 0; j < 8; j++)
+                    if (j * 32 + lane < a.head_dim) acc[j] = wi == 0.0f ? acc[j] : fmaf(o[j * 32 + lane], wi, acc[j]);
+            }
         }
+        l = warp_sum(l);
+        if (parts > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 8; j++) part[warp][j * 32 + lane] = acc[j];
+            if (lane == 0) part_l[warp] = l;
+            __syncthreads();
+            if (warp % parts != 0) continue;
+            for (unsigned y = 1; y < parts; y++) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) acc[j] += part[warp + y][j * 32 + lane];
+                l += part_l[warp + y];
+            }
+        }
+        if (!in) continue;
+        const unsigned flat = block * a.block_rows + r, node = flat / a.group, head = kv_head * a.group + flat % a.group;
         T* dst = static_cast<T*>(a.out) + static_cast<size_t>(q.row0 + node) * a.out_stride + static_cast<size_t>(head) * a.head_dim;
 #pragma unroll
         for (int j = 0; j < 8; j++)

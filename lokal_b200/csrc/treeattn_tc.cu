@@ -4,38 +4,70 @@
 // Bound by memory up to about 250 query rows per key head (a key and its value are 4 * head_dim bytes and cost
 // 4 * head_dim flops per row; the measured 1634 TFLOP/s over 6570 GB/s are 249 flops per byte), so the aim is that the
 // copies never wait. One CTA per SM, 128 query rows by 128 keys:
-//   warp 8      brings K and V tiles, page by page, into a ring of stages with TMA (128-byte swizzle)
-//   warp 9      issues the products: S = Q K^T into TMEM, O += P V with P read from TMEM and V as it lies (MN-major)
-//   warps 0-3   take the even tiles, warps 4-7 the odd ones: S from TMEM, maximum, exp2, P back over S
+//   warp 8       brings K tiles, page by page, into a ring with TMA (128-byte swizzle)
+//   warp 9       issues S = Q K^T into TMEM
+//   warp 10      issues O += P V, with P read from TMEM and V as it lies (MN-major)
+//   warp 11      loads the query rows of the next block once the last scores of this one are there, and brings V tiles
+//   warps 0-3    take the even tiles, warps 4-7 the odd ones: S from TMEM, maximum, exp2, P back over S
 // The two groups of warps are two streams of the running softmax, each with a maximum, a sum and an accumulator of its
-// own, so neither waits for the other, and the product of one tile runs while the other group works on its own; they
-// are put together when the block ends. An accumulator is rescaled only when the maximum has grown by more than 2^8
-// since it was last set: weights then stay below 2^8, which neither 16-bit type nor the f32 sums mind.
+// own, so neither waits for the other; they are put together when the block ends. With head size 64, TMEM has room for a
+// third S, and the scores of a tile are ready when its group has done the one before; with 128 it is two. The end of a
+// block (its last products, then the way out) is hidden behind the scores of the next block's first tiles. The two kinds
+// of products have a warp each because issuing them is what costs: one warp for both took 2150 clocks a tile of head size
+// 64, half as much again as the copy of the tile. So have the copies: a tile's boxes took one warp 600 clocks for K, 600 for V.
+// K and V tiles have their places in one ring in the order of their use.
+// An accumulator is rescaled only when the maximum has grown by more than 2^8 since it was last set: weights then stay
+// below 2^8, which neither 16-bit type nor the f32 sums mind.
 // Weights are rounded to the cache's type for the product (half a step each, as the values they multiply were); sums,
 // maxima and scores are f32.
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "treeattn.cuh"
 
 namespace lokal {
 namespace {
 
-constexpr int kTcRows = 128, kTcKeys = 128, kTcThreads = 320;
-constexpr int kSoftmaxThreads = 256;
+constexpr int kTcRows = 128, kTcKeys = 128, kTcThreads = 384;
 
 template <int HD>
 struct TcShape {
-    static constexpr int kSubs = HD / 64;                   // 64-column panels of 128 bytes
-    static constexpr unsigned kPanel = 128 * 128;           // bytes of a panel of 128 rows
-    static constexpr unsigned kTile = kSubs * kPanel;       // bytes of a K or V tile, and of Q
-    static constexpr int kStages = HD == 128 ? 3 : 6;       // 192 KB either way
-    static constexpr unsigned kMl = kTile + kStages * 2 * kTile;        // float2[2][128]
-    static constexpr unsigned kBars = kMl + 2 * 128 * 8;                // mbarriers
-    static constexpr unsigned kNumBars = (3 * kStages + 6 + 1) / 2 * 2;
-    static constexpr unsigned kMisc = kBars + kNumBars * 8;             // TMEM address, flags
+    static constexpr int kSubs = HD / 64;             // 64-column panels of 128 bytes
+    static constexpr unsigned kPanel = 128 * 128;     // bytes of a panel of 128 rows
+    static constexpr unsigned kTile = kSubs * kPanel; // bytes of a K or V tile, and of Q
+    static constexpr unsigned kSlots = HD == 128 ? 6 : 13;  // K and V tiles in the ring: 192 / 208 KB beside Q
+    static constexpr unsigned kScores = HD == 128 ? 2 : 3;  // S tiles in TMEM: 128 columns each, beside two accumulators of HD
+    static constexpr unsigned kAhead = kScores - 1;         // tiles whose scores are computed before a tile's output product
+    static constexpr unsigned kRing = kTile;
+    static constexpr unsigned kMl = kRing + kSlots * kTile;  // float2[2][128]
+    static constexpr unsigned kBars = kMl + 2 * 128 * 8;     // mbarriers
+    static constexpr unsigned kNumBars = 2 * kSlots + 3 * kScores + 3;
+    static constexpr unsigned kMisc = kBars + (kNumBars + 1) / 2 * 16;  // TMEM address, flags
     static constexpr unsigned kBytes = kMisc + 32;
     static_assert(kBytes <= 227 * 1024, "a CTA's shared memory");
+    static_assert(kScores * 128 + 2 * HD <= 512, "TMEM columns");
 };
+
+// A slot of the ring and the parity of its round.
+template <int HD>
+struct RingAt {
+    unsigned slot = 0, round = 0;
+    __device__ __forceinline__ void add(unsigned k) {  // at most a round
+        slot += k;
+        if (slot >= TcShape<HD>::kSlots) {
+            slot -= TcShape<HD>::kSlots;
+            round ^= 1u;
+        }
+    }
+};
+
+// Place of a block's tiles in the order of their use, counted from the block's first: K of the first kAhead tiles, then K of
+// each further tile and V of the one kAhead before it, then the V tiles that are left.
+template <int HD>
+__device__ __forceinline__ unsigned v_place(unsigned i, unsigned n) {
+    return min(i + TcShape<HD>::kAhead + 1u, n) + i;
+}
 
 // ---- tcgen05 ----
 __device__ __forceinline__ void tc_alloc(uint32_t dst, unsigned cols) {
@@ -50,9 +82,15 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void tc_commit(uint32_t mbar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mbar) : "memory");
 }
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// One lane of a warp, always the same.
+__device__ __forceinline__ bool tc_elect() {
+    unsigned yes;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(yes));
+    return yes != 0;
+}
 
 // D[tmem] (+)= A[smem] B[smem]
 __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
@@ -78,6 +116,14 @@ __device__ __forceinline__ void tc_ld32(uint32_t at, uint32_t (&v)[32]) {
         "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
         : TC_R4(v, 0), TC_R4(v, 4), TC_R4(v, 8), TC_R4(v, 12), TC_R4(v, 16), TC_R4(v, 20), TC_R4(v, 24), TC_R4(v, 28)
         : "r"(at));
+}
+// Waits for the warp's loads; naming the registers keeps their uses behind it.
+#define TC_RW4(v, i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3])
+__device__ __forceinline__ void tc_wait_ld(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : TC_RW4(v, 0), TC_RW4(v, 4), TC_RW4(v, 8), TC_RW4(v, 12), TC_RW4(v, 16), TC_RW4(v, 20), TC_RW4(v, 24), TC_RW4(v, 28)
+                 :
+                 : "memory");
 }
 __device__ __forceinline__ void tc_st32(uint32_t at, const uint32_t (&v)[32]) {
     asm volatile(
@@ -137,6 +183,12 @@ __device__ __forceinline__ bool bad_pair(uint32_t v) {
     return (v & e) == e || ((v >> 16) & e) == e;
 }
 
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t mbar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(mbar)
+                 : "memory");
+}
+
 // A wait that gives up: after `limit` polls, or when another role of the CTA has.
 __device__ __forceinline__ bool tc_wait(uint32_t mbar, unsigned parity, unsigned limit, volatile int* gave_up) {
     if (mbar_try_wait(mbar, parity)) return true;
@@ -182,323 +234,246 @@ __device__ __noinline__ void add_bad_values(const TreeArgs& a, const TreeUnit& u
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1)
-    tree_attn_tc_kernel(const TreeArgs a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    tree_attn_tc_kernel(const TreeArgs a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                        const __grid_constant__ CUtensorMap map_v) {
     using S = TcShape<HD>;
     extern __shared__ __align__(1024) unsigned char tc_smem[];
     const uint32_t smem = smem_addr(tc_smem);
     const unsigned tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     const uint32_t bars = smem + S::kBars;
-    auto kfull = [&](int st) { return bars + st * 8; };
-    auto vfull = [&](int st) { return bars + (S::kStages + st) * 8; };
-    auto empty = [&](int st) { return bars + (2 * S::kStages + st) * 8; };
-    const uint32_t sfull = bars + 3 * S::kStages * 8, pready = sfull + 16, qfull = sfull + 32, udone = sfull + 40;
-    volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(tc_smem + S::kMisc);  // [0] TMEM, [1] a wait gave up, [2], [3] bad values in a unit
+    const auto full = [&](unsigned slot) { return bars + slot * 8; };
+    const auto empty = [&](unsigned slot) { return bars + (S::kSlots + slot) * 8; };
+    const auto sfull = [&](unsigned b) { return bars + (2 * S::kSlots + b) * 8; };                  // scores are there
+    const auto pready = [&](unsigned b) { return bars + (2 * S::kSlots + S::kScores + b) * 8; };    // weights are there
+    const auto sfree = [&](unsigned b) { return bars + (2 * S::kSlots + 2 * S::kScores + b) * 8; };  // weights have been used
+    const uint32_t qfull = bars + (2 * S::kSlots + 3 * S::kScores) * 8, qfree = qfull + 8, udone = qfull + 16;  // udone: the last product of a block
+    volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(tc_smem + S::kMisc);  // [0] TMEM, [1] a wait gave up, [2..5] bad values, by block
     volatile int* gave_up = reinterpret_cast<volatile int*>(misc + 1);
     float2* ml = reinterpret_cast<float2*>(tc_smem + S::kMl);
     // set-up that touches no global memory goes ahead of the wait for the launch before
     if (warp == 8) {
         tc_alloc(smem + S::kMisc, 512);
         if (lane == 0) {
-            for (int st = 0; st < S::kStages; st++) {
-                mbar_init(kfull(st), 1);
-                mbar_init(vfull(st), 1);
-                mbar_init(empty(st), 1);
+            for (unsigned i = 0; i < 2 * S::kSlots + S::kScores; i++) mbar_init(bars + i * 8, 1);
+            for (unsigned b = 0; b < S::kScores; b++) {
+                mbar_init(pready(b), 128);
+                mbar_init(sfree(b), 1);
             }
-            for (int w = 0; w < 2; w++) {
-                mbar_init(sfull + 8 * w, 1);
-                mbar_init(pready + 8 * w, 128);
-            }
-            mbar_init(qfull, kSoftmaxThreads);
+            mbar_init(qfull, 1);
+            mbar_init(qfree, 1);
             mbar_init(udone, 1);
             mbar_init_fence();
-            misc[1] = misc[2] = misc[3] = 0;
+            for (int i = 1; i < 6; i++) misc[i] = 0;
         }
     }
     pdl_sync();
-    // the ring is not in use yet: it holds the sums of the walk
+    // the ring is not in use yet: its first bytes hold the sums of the walk
     const unsigned shares = gridDim.x;
-    const TreePlace place = tree_locate<kTcRows, kTcKeys, kTcThreads>(a, reinterpret_cast<unsigned long long*>(tc_smem), blockIdx.x == 0, [&](unsigned long long total) {
-        const unsigned g = total < shares ? static_cast<unsigned>(total) : shares;
-        return blockIdx.x < g ? tree_share(total, blockIdx.x, g) : total;
+    const TreePlace place = tree_locate<kTcKeys, kTcThreads>(a, reinterpret_cast<unsigned long long*>(tc_smem), blockIdx.x == 0, [&](unsigned total) {
+        const TreeShares s(total, shares);
+        return blockIdx.x < s.g ? s.first(blockIdx.x) : total;
     });
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = misc[0];
-    const unsigned g = place.total < shares ? static_cast<unsigned>(place.total) : shares;
-    TreeWalk<kTcRows, kTcKeys> walk;
-    walk.start(a, place, place.seq < a.n_seqs ? tree_share(place.total, blockIdx.x, g) : 0, place.seq < a.n_seqs ? tree_share(place.total, blockIdx.x + 1, g) : 0);
-    TreeUnit u;
+    const TreeShares share(place.total, shares);
     bool ok = place.seq < a.n_seqs;
+    TreeWalk<kTcKeys> walk;
+    walk.start(a, place, ok ? share.first(blockIdx.x) : 0u, ok ? share.first(blockIdx.x + 1) : 0u);
+    TreeUnit u;
 
-    if (warp == 8) {
-        // ---- K and V tiles ----
-        unsigned t = 0;  // tiles so far
+    if (warp == 8 || warp == 11) {
+        // ---- K tiles (warp 8), query rows and V tiles (warp 11) ----
+        const bool is_k = warp == 8;
+        const CUtensorMap* map = is_k ? &map_k : &map_v;
         const unsigned box_rows = min(a.page_rows, static_cast<unsigned>(kTcKeys));
+        RingAt<HD> at;
+        bool reused = false;               // the ring has been round once
+        unsigned units = 0, issued = 0, parity = 0;  // blocks; by slot: whether it was filled, and in which round
         while (ok && walk.next(a, u)) {
-            for (unsigned kt = u.k0; ok && kt < u.k1; kt++, t++) {
-                const int st = static_cast<int>(t % S::kStages);
-                const unsigned round = t / S::kStages;
-                if (round) ok = tc_wait(empty(st), (round - 1) & 1u, a.wait_limit, gave_up);
-                ok = __all_sync(0xffffffffu, ok);
+            const unsigned n = u.k1 - u.k0;
+            // lane b names the page of box b of a tile; the next tile's page is on its way while this tile is copied
+            const auto row_of = [&](unsigned i) -> int {
+                const unsigned pos = (u.k0 + i) * kTcKeys + lane * box_rows;
+                if (i >= n || lane * box_rows >= kTcKeys || pos >= static_cast<unsigned>(u.seq.len)) return 0;
+                return static_cast<int>((tree_page(a, u.seq.slot, pos >> a.page_shift) << a.page_shift) + (pos & (a.page_rows - 1)));
+            };
+            int y = row_of(0);
+            if (!is_k) {
+                if (units) ok = __all_sync(0xffffffffu, tc_wait(qfree, (units - 1) & 1u, a.wait_limit, gave_up));
                 if (!ok) break;
-                const unsigned pos0 = kt * kTcKeys, left = static_cast<unsigned>(u.seq.len) - pos0;
-                const unsigned boxes = (min(left, static_cast<unsigned>(kTcKeys)) + box_rows - 1) / box_rows;
                 if (lane == 0) {
-                    mbar_expect_tx(kfull(st), boxes * box_rows * 128 * S::kSubs);
-                    mbar_expect_tx(vfull(st), boxes * box_rows * 128 * S::kSubs);
+                    const unsigned nodes = kTcRows / a.group;
+                    mbar_expect_tx(qfull, nodes * a.group * 128 * S::kSubs);
+#pragma unroll
+                    for (int c = 0; c < S::kSubs; c++)
+                        tma_load_3d(smem + c * S::kPanel, &map_q, c * 64, static_cast<int>(u.kv_head * a.group), static_cast<int>(u.seq.row0 + u.block * nodes), qfull);
                 }
+                __syncwarp();
+                units++;
+            }
+            unsigned behind = is_k ? 0u : v_place<HD>(0, n);
+            reused |= at.slot + behind >= S::kSlots;
+            at.add(behind);
+            const int x = static_cast<int>(u.kv_head * HD);
+            for (unsigned i = 0; i < n; i++) {
+                if (reused) ok = __all_sync(0xffffffffu, tc_wait(empty(at.slot), at.round ^ 1u, a.wait_limit, gave_up));
+                if (!ok) break;
+                const unsigned left = static_cast<unsigned>(u.seq.len) - (u.k0 + i) * kTcKeys;
+                const unsigned boxes = (min(left, static_cast<unsigned>(kTcKeys)) + box_rows - 1) / box_rows;
+                issued |= 1u << at.slot;
+                parity = (parity & ~(1u << at.slot)) | (at.round << at.slot);
+                if (lane == 0) mbar_expect_tx(full(at.slot), boxes * box_rows * 128 * S::kSubs);
                 __syncwarp();
                 if (lane < boxes) {
-                    const unsigned pos = pos0 + lane * box_rows;
-                    const int y = static_cast<int>((tree_page(a, u.seq.slot, pos >> a.page_shift) << a.page_shift) + (pos & (a.page_rows - 1)));
-                    const int x = static_cast<int>(u.kv_head * HD);
-                    const uint32_t k_at = smem + S::kTile + st * 2 * S::kTile + lane * box_rows * 128, v_at = k_at + S::kTile;
+                    const uint32_t to = smem + S::kRing + at.slot * S::kTile + lane * box_rows * 128;
 #pragma unroll
-                    for (int s = 0; s < S::kSubs; s++) tma_load_2d(k_at + s * S::kPanel, &map_k, x + s * 64, y, kfull(st));
-#pragma unroll
-                    for (int s = 0; s < S::kSubs; s++) tma_load_2d(v_at + s * S::kPanel, &map_v, x + s * 64, y, vfull(st));
+                    for (int c = 0; c < S::kSubs; c++) tma_load_2d(to + c * S::kPanel, map, x + c * 64, y, full(at.slot));
                 }
-                __syncwarp();
+                y = row_of(i + 1);
+                const unsigned next = i + 1 == n ? 2 * n : is_k ? i + 1 + (i + 1 > S::kAhead ? i + 1 - S::kAhead : 0u) : v_place<HD>(i + 1, n);
+                reused |= at.slot + (next - behind) >= S::kSlots;
+                at.add(next - behind);
+                behind = next;
             }
         }
-        if (!ok) {
+        if (!ok && place.seq < a.n_seqs) {
             // what is in flight lands before the CTA gives its memory back
-            for (int st = 0; st < S::kStages; st++) {
-                const unsigned n = t > static_cast<unsigned>(st) ? (t - 1 - st) / S::kStages : 0u;
-                if (t > static_cast<unsigned>(st)) {
-                    mbar_wait_bounded(kfull(st), n & 1u, a.wait_limit);
-                    mbar_wait_bounded(vfull(st), n & 1u, a.wait_limit);
-                }
-            }
+            for (unsigned slot = 0; slot < S::kSlots; slot++)
+                if ((issued >> slot) & 1u) mbar_wait_bounded(full(slot), (parity >> slot) & 1u, a.wait_limit);
         }
     } else if (warp == 9) {
-        // ---- products ----
-        if (lane == 0) {
-            constexpr unsigned fmt = std::is_same<T, __half>::value ? 0u : 1u;
-            constexpr uint32_t id_s = tc_idesc(fmt, kTcKeys, 0), id_o = tc_idesc(fmt, HD, 1);
-            unsigned t = 0, units = 0, ended = 0;  // tiles, blocks begun, blocks whose last product has been issued
-            bool first[2] = {true, true};
-            // O += P V of tile x
-            auto product_v = [&](unsigned x, bool last) -> bool {
-                const unsigned w = x & 1u;
-                const int st = static_cast<int>(x % S::kStages);
-                if (!tc_wait(vfull(st), (x / S::kStages) & 1u, a.wait_limit, gave_up)) return false;
-                if (!tc_wait(pready + 8 * w, (x >> 1) & 1u, a.wait_limit, gave_up)) return false;
+        // ---- S = Q K^T ----
+        constexpr uint32_t idesc = tc_idesc(std::is_same<T, __half>::value ? 0u : 1u, kTcKeys, 0);
+        const uint64_t q_desc = tc_desc(smem, 16), k_desc = tc_desc(smem + S::kRing, 16);
+        RingAt<HD> at;                     // of the next K tile
+        unsigned b = 0, b_round = 0, t = 0, units = 0;  // S tile, key tiles, blocks
+        const auto wait = [&](uint32_t bar, unsigned parity) { ok = ok && __all_sync(0xffffffffu, tc_wait(bar, parity, a.wait_limit, gave_up)); };
+        while (ok && walk.next(a, u)) {
+            const unsigned n = u.k1 - u.k0;
+            wait(qfull, units & 1u);
+            for (unsigned i = 0; ok && i < n; i++) {
+                wait(full(at.slot), at.round);
+                if (t >= S::kScores) wait(sfree(b), b_round ^ 1u);  // the weights that these scores overwrite have been used
+                if (!ok) break;
                 tc_fence_after();
-                const uint32_t v_at = smem + S::kTile + st * 2 * S::kTile + S::kTile;
-#pragma unroll
-                for (int k = 0; k < kTcKeys / 16; k++)
-                    tc_mma_ts(tmem + 256 + w * HD, tmem + w * 128 + k * 8, tc_desc(v_at + k * 2048, S::kPanel), id_o, !(first[w] && k == 0));
-                first[w] = false;
-                tc_commit(empty(st));
-                if (last) {
-                    tc_commit(udone);
-                    ended++;
-                }
-                return true;
-            };
-            while (ok && walk.next(a, u)) {
-                if (t) ok = product_v(t - 1, true);
-                first[0] = first[1] = true;
-                if (ok) ok = tc_wait(qfull, units & 1u, a.wait_limit, gave_up);
-                units++;
-                for (unsigned kt = u.k0; ok && kt < u.k1; kt++, t++) {
-                    const int st = static_cast<int>(t % S::kStages);
-                    ok = tc_wait(kfull(st), (t / S::kStages) & 1u, a.wait_limit, gave_up);
-                    // Products of one shape run in the order of their issue, so this one comes after the product that
-                    // reads the weights it overwrites; of two shapes that is not said, and the earlier one is waited for.
-                    if (HD != 128 && ok && t >= 2) ok = tc_wait(empty(static_cast<int>((t - 2) % S::kStages)), ((t - 2) / S::kStages) & 1u, a.wait_limit, gave_up);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t k_at = smem + S::kTile + st * 2 * S::kTile;
+                if (tc_elect()) {
+                    const uint64_t kd = k_desc + at.slot * (S::kTile >> 4);
 #pragma unroll
                     for (int k = 0; k < HD / 16; k++) {
-                        const unsigned off = (k / 4) * S::kPanel + (k % 4) * 32;
-                        tc_mma_ss(tmem + (t & 1u) * 128, tc_desc(smem + off, 16), tc_desc(k_at + off, 16), id_s, k != 0);
+                        const unsigned off = ((k / 4) * S::kPanel + (k % 4) * 32) >> 4;
+                        tc_mma_ss(tmem + b * 128, q_desc + off, kd + off, idesc, k != 0);
                     }
-                    tc_commit(sfull + 8 * (t & 1u));
-                    if (kt > u.k0) ok = product_v(t - 1, false);
+                    tc_commit(sfull(b));
+                    tc_commit(empty(at.slot));
+                    if (i == n - 1) tc_commit(qfree);
                 }
+                __syncwarp();
+                if (++b == S::kScores) {
+                    b = 0;
+                    b_round ^= 1u;
+                }
+                t++;
+                at.add(i + 1 < n ? (i < S::kAhead ? 1u : 2u) : n + 1 - (n > S::kAhead + 1 ? n - 1 - S::kAhead : 0u));
             }
-            if (ok && t) ok = product_v(t - 1, true);
-            if (!ok && t) {
-                // the products in flight end before TMEM is given back
-                tc_commit(udone);
-                mbar_wait_bounded(udone, ended & 1u, a.wait_limit);
-            }
+            units++;
         }
-        __syncwarp();
+        if (!ok && place.seq < a.n_seqs) {
+            // the products in flight end before TMEM is given back
+            if (t) mbar_wait_bounded(sfull((t - 1) % S::kScores), ((t - 1) / S::kScores) & 1u, a.wait_limit);
+        }
+    } else if (warp == 10) {
+        // ---- O += P V ----
+        constexpr uint32_t idesc = tc_idesc(std::is_same<T, __half>::value ? 0u : 1u, HD, 1);
+        const uint64_t v_desc = tc_desc(smem + S::kRing, S::kPanel);
+        RingAt<HD> at;
+        unsigned b = 0, b_round = 0, t = 0, units = 0;
+        const auto wait = [&](uint32_t bar, unsigned parity) { ok = ok && __all_sync(0xffffffffu, tc_wait(bar, parity, a.wait_limit, gave_up)); };
+        while (ok && walk.next(a, u)) {
+            const unsigned n = u.k1 - u.k0;
+            unsigned begun = 0;  // bit w: stream w of the block has something in its accumulator
+            unsigned behind = v_place<HD>(0, n);
+            at.add(behind);
+            for (unsigned i = 0; ok && i < n; i++) {
+                wait(full(at.slot), at.round);
+                wait(pready(b), b_round);
+                if (!ok) break;
+                tc_fence_after();
+                const unsigned w = t & 1u;
+                if (tc_elect()) {
+                    const uint64_t vd = v_desc + at.slot * (S::kTile >> 4);
+#pragma unroll
+                    for (int k = 0; k < kTcKeys / 16; k++)
+                        tc_mma_ts(tmem + S::kScores * 128 + w * HD, tmem + b * 128 + k * 8, vd + k * (2048 >> 4), idesc, k != 0 || (begun >> w) & 1u);
+                    tc_commit(sfree(b));
+                    tc_commit(empty(at.slot));
+                    if (i == n - 1) tc_commit(udone);
+                }
+                __syncwarp();
+                begun |= 1u << w;
+                if (++b == S::kScores) {
+                    b = 0;
+                    b_round ^= 1u;
+                }
+                t++;
+                const unsigned next = i + 1 < n ? v_place<HD>(i + 1, n) : 2 * n;
+                at.add(next - behind);
+                behind = next;
+            }
+            if (ok) units++;
+        }
+        if (!ok && place.seq < a.n_seqs) {
+            // the products in flight end before TMEM is given back
+            if (tc_elect()) tc_commit(udone);
+            mbar_wait_bounded(udone, units & 1u, a.wait_limit);
+        }
     } else {
         // ---- softmax ----
         const unsigned w = warp >> 2, row = tid & 127u;
         const uint32_t lanes = (warp & 3u) << 21;  // the warp's 32 lanes of TMEM
-        const uint32_t s_at = tmem + w * 128 + lanes, o_at = tmem + 256 + w * HD + lanes;
-        const float scale = fabsf(a.scale_log2);
-        const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;  // a negative scale turns q's sign
-        auto load_q = [&](const TreeUnit& x) {
-            const unsigned flat0 = x.block * kTcRows, rows_all = x.seq.n * a.group;
-#pragma unroll 4
-            for (unsigned e = tid; e < 128u * HD / 8; e += kSoftmaxThreads) {
-                const unsigned r = e / (HD / 8), c = e % (HD / 8);
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (flat0 + r < rows_all) {
-                    const unsigned flat = flat0 + r, node = flat / a.group, head = x.kv_head * a.group + flat % a.group;
-                    v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + static_cast<size_t>(x.seq.row0 + node) * a.q_stride + static_cast<size_t>(head) * HD + c * 8);
-                    v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-                }
-                *reinterpret_cast<uint4*>(tc_smem + (c / 8) * S::kPanel + r * 128 + (((c % 8) ^ (r & 7u)) << 4)) = v;
-            }
-            proxy_fence();
-            mbar_arrive(qfull);
-        };
-        unsigned t = 0, units = 0;
-        bool have = ok && walk.next(a, u);
-        if (have) load_q(u);
-        while (have) {
-            const unsigned flat0 = u.block * kTcRows, m_rows = min(static_cast<unsigned>(kTcRows), u.seq.n * a.group - flat0);
-            const bool busy = (warp & 3u) * 32 < m_rows;  // some row of the warp is there
-            const unsigned flat = flat0 + min(row, m_rows - 1), node = flat / a.group;
-            float m = -INFINITY, l = 0.0f;
-            bool begun = false;  // a tile of this stream has gone into the accumulator
-            for (unsigned kt = u.k0; ok && kt < u.k1; kt++, t++) {
-                if ((t & 1u) != w) continue;
-                ok = __all_sync(0xffffffffu, tc_wait(sfull + 8 * w, (t >> 1) & 1u, a.wait_limit, gave_up));
-                if (!ok) break;
-                tc_fence_after();
-                const int pos0 = static_cast<int>(kt) * kTcKeys;
-                const bool masked = pos0 + kTcKeys > u.seq.ctx;  // drafted rows, or the end, are in the tile
-                if (busy) {
-                    unsigned bits[4];
-                    if (masked) {
-#pragma unroll
-                        for (int j = 0; j < 4; j++) bits[j] = tree_visible(a, u.seq, node, pos0 + 32 * j);
-                    }
-                    uint32_t v[32];
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        tc_ld32(s_at + 32 * j, v);
-                        tc_wait_ld();
-                        if (masked) {
-#pragma unroll
-                            for (int i = 0; i < 32; i++) top = (bits[j] >> i) & 1u ? fmaxf(top, __uint_as_float(v[i])) : top;
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 32; i++) top = fmaxf(top, __uint_as_float(v[i]));
-                        }
-                    }
-                    if (top != -INFINITY) top *= scale;
-                    const float before = m;
-                    if (!begun) {
-                        m = top;
-                    } else if (__any_sync(0xffffffffu, top > m + 8.0f)) {
-                        m = fmaxf(m, top);
-                        const float f = before == -INFINITY ? 0.0f : ex2(before - m);
-                        l *= f;
-#pragma unroll
-                        for (int j = 0; j < HD / 32; j++) {
-                            tc_ld32(o_at + 32 * j, v);
-                            tc_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                            tc_st32(o_at + 32 * j, v);
-                        }
-                    }
-                    const float ref = m == -INFINITY ? 0.0f : m;
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        tc_ld32(s_at + 32 * j, v);
-                        tc_wait_ld();
-                        uint32_t p[16];
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            float lo = ex2(fmaf(__uint_as_float(v[2 * i]), scale, -ref)), hi = ex2(fmaf(__uint_as_float(v[2 * i + 1]), scale, -ref));
-                            if (masked) {
-                                lo = (bits[j] >> (2 * i)) & 1u ? lo : 0.0f;
-                                hi = (bits[j] >> (2 * i + 1)) & 1u ? hi : 0.0f;
-                            }
-                            sum[i & 3] += lo + hi;
-                            p[i] = pack2<T>(lo, hi);
-                        }
-                        tc_st16(s_at + 16 * j, p);
-                    }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tc_wait_st();
-                }
-                begun = true;
-                if (masked) {
-                    // V rows behind the last position are cleared (they may hold anything, and 0 * NaN is NaN); so are drafted
-                    // ones with an infinity or a NaN, which rows that do not see them must not get: add_bad_values
-                    const int st = static_cast<int>(t % S::kStages);
-                    ok = __all_sync(0xffffffffu, tc_wait(vfull(st), (t / S::kStages) & 1u, a.wait_limit, gave_up));
-                    unsigned char* v_at = tc_smem + S::kTile + st * 2 * S::kTile + S::kTile;
-                    const int valid = min(kTcKeys, u.seq.len - pos0), drafted = max(0, u.seq.ctx - pos0);
-                    const unsigned quads = S::kSubs * 8;  // 16-byte pieces of a row
-                    for (unsigned e = row; ok && e < (kTcKeys - valid) * quads; e += 128) {
-                        const unsigned r = valid + e / quads, c = e % quads;
-                        *reinterpret_cast<uint4*>(v_at + (c / 8) * S::kPanel + r * 128 + (c % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    }
-                    // eight threads to a panel row: a row is cleared by the threads that read it
-                    const unsigned g8 = row >> 3, c8 = row & 7u;
-                    for (int r0 = drafted; r0 < valid; r0 += 16) {
-                        const int r = r0 + static_cast<int>(g8);
-                        bool bad = false;
-                        if (ok && r < valid) {
-#pragma unroll
-                            for (int s = 0; s < S::kSubs; s++) {
-                                const uint4 x = *reinterpret_cast<const uint4*>(v_at + s * S::kPanel + r * 128 + c8 * 16);
-                                bad = bad || bad_pair<T>(x.x) || bad_pair<T>(x.y) || bad_pair<T>(x.z) || bad_pair<T>(x.w);
-                            }
-                        }
-                        const unsigned who = __ballot_sync(0xffffffffu, bad);
-                        if (who == 0) continue;
-                        if ((who >> (lane & 24u)) & 0xffu) {
-#pragma unroll
-                            for (int s = 0; s < S::kSubs; s++) *reinterpret_cast<uint4*>(v_at + s * S::kPanel + r * 128 + c8 * 16) = make_uint4(0u, 0u, 0u, 0u);
-                            misc[2 + (units & 1u)] = 1;
-                        }
-                    }
-                    proxy_fence();
-                }
-                tc_fence_before();
-                mbar_arrive(pready + 8 * w);
-            }
-            // every S of the unit has been read, so Q is free
-            bar_softmax();
-            const TreeUnit done = u;
-            have = walk.next(a, u);
-            if (have) load_q(u);
-            ok = ok && tc_wait(udone, units & 1u, a.wait_limit, gave_up);
+        const uint32_t o_at = tmem + S::kScores * 128 + lanes;
+        const float scale = a.scale_log2;
+        unsigned t = 0, seq0 = 0, units = 0;  // key tiles, ring tiles and blocks before the block
+        // the block that is done but not yet written
+        TreeUnit last{};
+        float last_m = 0.0f, last_l = 0.0f;
+        bool pending = false;
+        // The two streams of a block are put together and written out.
+        const auto finish = [&] {
+            const unsigned which = units - 1;  // the block's number
+            const unsigned flat0 = last.block * a.block_rows, m_rows = min(a.block_rows, last.seq.n * a.group - flat0);
+            ok = __all_sync(0xffffffffu, ok && tc_wait(udone, which & 1u, a.wait_limit, gave_up));
             tc_fence_after();
-            ml[w * 128 + row] = make_float2(m, l);
+            ml[w * 128 + row] = make_float2(last_m, last_l);
             bar_softmax();
-            const bool fix = misc[2 + (units & 1u)] != 0;
+            const bool fix = misc[2 + (which & 3u)] != 0;
+            if (tid == 0) misc[2 + ((which + 2) & 3u)] = 0;  // read two blocks ago, written again only behind the barrier below
             const float2 other = ml[(w ^ 1u) * 128 + row];
-            // the two streams together: weights of each accumulator, 0 for one that saw nothing (it may never have been written)
-            const float top = fmaxf(m, other.x), ref = top == -INFINITY ? 0.0f : top;
-            const float f_own = l == 0.0f ? 0.0f : ex2(m - ref), f_other = other.y == 0.0f ? 0.0f : ex2(other.x - ref);
-            const float total = (l == 0.0f ? 0.0f : l * f_own) + (other.y == 0.0f ? 0.0f : other.y * f_other);
+            // weights of the two accumulators, 0 for one that saw nothing (it may never have been written)
+            const float top = fmaxf(last_m, other.x), ref = top == -INFINITY ? 0.0f : top;
+            const float f_own = last_l == 0.0f ? 0.0f : ex2(last_m - ref), f_other = other.y == 0.0f ? 0.0f : ex2(other.x - ref);
+            const float total = (last_l == 0.0f ? 0.0f : last_l * f_own) + (other.y == 0.0f ? 0.0f : other.y * f_other);
             const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-            if (busy) {
-                const unsigned head = done.kv_head * a.group + flat % a.group;
-                T* out = static_cast<T*>(a.out) + static_cast<size_t>(done.seq.row0 + node) * a.out_stride + static_cast<size_t>(head) * HD;
-                const size_t piece = ((static_cast<size_t>(blockIdx.x) * 2 + done.piece) * kTcRows + row);
+            if ((warp & 3u) * 32 < m_rows) {
+                const unsigned flat = flat0 + min(row, m_rows - 1), node = flat / a.group, head = last.kv_head * a.group + flat % a.group;
+                T* out = static_cast<T*>(a.out) + static_cast<size_t>(last.seq.row0 + node) * a.out_stride + static_cast<size_t>(head) * HD;
+                const size_t piece = (static_cast<size_t>(blockIdx.x) * 2 + last.piece) * kTcRows + row;
                 float* po = a.part_o + piece * HD;
                 const unsigned c0 = w * (HD / 2);
 #pragma unroll
                 for (int j = 0; j < HD / 64; j++) {
                     uint32_t x[32], y[32];
-                    tc_ld32(tmem + 256 + w * HD + lanes + c0 + 32 * j, x);
-                    tc_ld32(tmem + 256 + (w ^ 1u) * HD + lanes + c0 + 32 * j, y);
-                    tc_wait_ld();
+                    tc_ld32(o_at + w * HD + c0 + 32 * j, x);
+                    tc_ld32(o_at + (w ^ 1u) * HD + c0 + 32 * j, y);
+                    tc_wait_ld(x);
+                    tc_wait_ld(y);
                     float o[32];
 #pragma unroll
                     for (int i = 0; i < 32; i++)
-                        o[i] = fmaf(l == 0.0f ? 0.0f : __uint_as_float(x[i]), f_own, other.y == 0.0f ? 0.0f : __uint_as_float(y[i]) * f_other);
+                        o[i] = fmaf(last_l == 0.0f ? 0.0f : __uint_as_float(x[i]), f_own, other.y == 0.0f ? 0.0f : __uint_as_float(y[i]) * f_other);
                     if (row < m_rows) {
-                        if (done.whole) {
+                        if (last.whole) {
 #pragma unroll
                             for (int i = 0; i < 32; i += 8)
                                 *reinterpret_cast<uint4*>(out + c0 + 32 * j + i) =
@@ -512,13 +487,167 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
                 if (row < m_rows) {
-                    if (!done.whole && w == 0) a.part_ml[piece] = make_float2(top, total);
-                    if (fix && total != 0.0f) add_bad_values<T, HD>(a, done, node, head, ref, total, out, done.whole ? nullptr : po, c0, c0 + HD / 2);
+                    if (!last.whole && w == 0) a.part_ml[piece] = make_float2(top, total);
+                    if (fix && total != 0.0f) add_bad_values<T, HD>(a, last, node, head, ref, total, out, last.whole ? nullptr : po, c0, c0 + HD / 2);
                 }
             }
             tc_fence_before();
-            if (tid == 0) misc[2 + ((units + 1) & 1u)] = 0;  // read a unit ago, written again only behind the barrier
-            bar_softmax();
+            bar_softmax();  // the accumulators may be written again
+            pending = false;
+        };
+        float m = 0.0f, l = 0.0f;  // of the block, for this stream
+        bool begun = false;        // a tile of this stream has gone into the accumulator
+        // A row's 128 scores to weights, in two passes of 32 at a time with the next 32 on their way: the maximum, then the
+        // weights. MASKED: drafted rows, or the end, are in the tile.
+        const auto weigh = [&](auto masked_, uint32_t s_at, unsigned i, const unsigned (&bits)[4]) {
+            constexpr bool MASKED = decltype(masked_)::value;
+            uint32_t v[2][32];
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tc_ld32(s_at, v[0]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t(&x)[32] = v[j & 1];
+                tc_wait_ld(x);
+                tc_ld32(s_at + 32 * ((j + 1) & 3), v[(j + 1) & 1]);  // after the last, the first again
+                if (MASKED) {
+#pragma unroll
+                    for (int c = 0; c < 32; c++) tops[c & 3] = (bits[j] >> c) & 1u ? fmaxf(tops[c & 3], __uint_as_float(x[c])) : tops[c & 3];
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 32; c += 8) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) tops[k] = fmaxf(fmaxf(tops[k], __uint_as_float(x[c + k])), __uint_as_float(x[c + k + 4]));
+                    }
+                }
+            }
+            float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+            if (top != -INFINITY) top *= scale;
+            if (__any_sync(0xffffffffu, top > m + 8.0f)) {
+                const float before = m;
+                m = fmaxf(m, top);
+                const float f = before == -INFINITY ? 0.0f : ex2(before - m);
+                l *= f;
+                if (begun) {
+                    // the stream's earlier product has to be in the accumulator
+                    const unsigned earlier = t + i - 2;
+                    ok = __all_sync(0xffffffffu, tc_wait(sfree(earlier % S::kScores), (earlier / S::kScores) & 1u, a.wait_limit, gave_up));
+                    tc_fence_after();
+                    for (int c = 0; c < HD / 32; c++) {
+                        uint32_t o[32];
+                        tc_ld32(o_at + w * HD + 32 * c, o);
+                        tc_wait_ld(o);
+#pragma unroll
+                        for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                        tc_st32(o_at + w * HD + 32 * c, o);
+                    }
+                }
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
+            const float2 scale2 = make_float2(scale, scale), ref2 = make_float2(-ref, -ref);
+            float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t(&x)[32] = v[j & 1];
+                tc_wait_ld(x);
+                if (j < 3) tc_ld32(s_at + 32 * (j + 1), v[(j + 1) & 1]);
+                uint32_t p[16];
+#pragma unroll
+                for (int c = 0; c < 16; c++) {
+                    float2 z = fma2(make_float2(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), scale2, ref2);
+                    z.x = ex2(z.x);
+                    z.y = ex2(z.y);
+                    if (MASKED) {
+                        z.x = (bits[j] >> (2 * c)) & 1u ? z.x : 0.0f;
+                        z.y = (bits[j] >> (2 * c + 1)) & 1u ? z.y : 0.0f;
+                    }
+                    sum[c & 1] = add2(sum[c & 1], z);
+                    p[c] = pack2<T>(z.x, z.y);
+                }
+                tc_st16(s_at + 16 * j, p);
+            }
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            tc_wait_st();
+        };
+        // V rows behind the last position are cleared (they may hold anything, and 0 * NaN is NaN); so are drafted ones with an
+        // infinity or a NaN, which rows that do not see them must not get: add_bad_values.
+        const auto clear_v = [&](unsigned i, unsigned n, int pos0) {
+            const unsigned at = seq0 + v_place<HD>(i, n), slot = at % S::kSlots;
+            ok = __all_sync(0xffffffffu, ok && tc_wait(full(slot), (at / S::kSlots) & 1u, a.wait_limit, gave_up));
+            if (!ok) return;
+            unsigned char* v_at = tc_smem + S::kRing + slot * S::kTile;
+            const int valid = min(kTcKeys, u.seq.len - pos0), drafted = max(0, u.seq.ctx - pos0);
+            const unsigned pieces = S::kSubs * 8;  // of 16 bytes, to a row
+            for (unsigned e = row; e < (kTcKeys - valid) * pieces; e += 128) {
+                const unsigned r = valid + e / pieces, c = e % pieces;
+                *reinterpret_cast<uint4*>(v_at + (c / 8) * S::kPanel + r * 128 + (c % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            // eight threads to a panel row: a row is cleared by the threads that read it
+            const unsigned g8 = row >> 3, c8 = row & 7u;
+            for (int r0 = drafted; r0 < valid; r0 += 16) {
+                const int r = r0 + static_cast<int>(g8);
+                bool bad = false;
+                if (r < valid) {
+#pragma unroll
+                    for (int c = 0; c < S::kSubs; c++) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(v_at + c * S::kPanel + r * 128 + c8 * 16);
+                        bad = bad || bad_pair<T>(x.x) || bad_pair<T>(x.y) || bad_pair<T>(x.z) || bad_pair<T>(x.w);
+                    }
+                }
+                const unsigned who = __ballot_sync(0xffffffffu, bad);
+                if ((who >> (lane & 24u)) & 0xffu) {
+#pragma unroll
+                    for (int c = 0; c < S::kSubs; c++) *reinterpret_cast<uint4*>(v_at + c * S::kPanel + r * 128 + c8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    misc[2 + (units & 3u)] = 1;
+                }
+            }
+            proxy_fence();
+        };
+        // Whether or not a wait has given up: the two groups meet at the barriers of every block.
+        for (;;) {
+            const bool more = walk.next(a, u);
+            if (!more && !pending) break;
+            const unsigned n = more ? u.k1 - u.k0 : 0u;
+            const unsigned flat0 = u.block * a.block_rows, m_rows = min(a.block_rows, u.seq.n * a.group - flat0);
+            m = -INFINITY;
+            l = 0.0f;
+            begun = false;
+            unsigned i = (t ^ w) & 1u;
+            do {
+                const unsigned b = (t + i) % S::kScores;
+                bool has = ok && i < n;
+                if (has) ok = has = __all_sync(0xffffffffu, tc_wait(sfull(b), ((t + i) / S::kScores) & 1u, a.wait_limit, gave_up));
+                if (has) {
+                    tc_fence_after();
+                    const int pos0 = static_cast<int>(u.k0 + i) * kTcKeys;
+                    const bool busy = (warp & 3u) * 32 < m_rows;  // some row of the warp is there
+                    unsigned bits[4];
+                    if (pos0 + kTcKeys <= u.seq.ctx) {
+                        if (busy) weigh(std::false_type{}, tmem + b * 128 + lanes, i, bits);
+                    } else {
+                        if (busy) {
+                            const unsigned node = (flat0 + min(row, m_rows - 1)) / a.group;
+#pragma unroll
+                            for (int j = 0; j < 4; j++) bits[j] = tree_visible(a, u.seq, node, pos0 + 32 * j);
+                            weigh(std::true_type{}, tmem + b * 128 + lanes, i, bits);
+                        }
+                        clear_v(i, n, pos0);
+                    }
+                    begun = true;
+                }
+                if (pending) finish();  // its last product ran while this tile's weights were worked out
+                if (has) {
+                    tc_fence_before();
+                    mbar_arrive(pready(b));
+                }
+                i += 2;
+            } while (i < n);
+            if (!more) break;
+            last = u;
+            last_m = m;
+            last_l = l;
+            pending = true;
+            t += n;
+            seq0 += 2 * n;
             units++;
         }
     }
@@ -556,13 +685,26 @@ bool encode_store(CUtensorMap* map, const TreeArgs& a, const char* base, bool ha
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// q as [row][query head][column], fetched as the rows of a block: the heads of one key head by 128 / group drafted rows.
+// What a box holds of another sequence's rows is computed and thrown away; behind the last row there are zeros.
+bool encode_q(CUtensorMap* map, const TreeArgs& a, bool half) {
+    const EncodeTiled enc = encode_tiled();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {a.head_dim, a.n_q_heads, a.rows};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(a.head_dim) * 2, a.q_stride * 2};
+    const cuuint32_t box[3] = {64, a.group, kTcRows / a.group}, step[3] = {1, 1, 1};
+    return enc(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a.q), dims, strides, box, step,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int HD>
 int launch_tc(lokal_cuda_ctx* ctx, cudaStream_t s, const TreeArgs& a) {
-    CUtensorMap map_k, map_v;
+    CUtensorMap map_q, map_k, map_v;
     constexpr bool half = std::is_same<T, __half>::value;
-    if (!encode_store(&map_k, a, a.k, half) || !encode_store(&map_v, a, a.v, half)) return ctx->fail(LOKAL_ERR_CUDA, "tree_attn: a store cannot be described to the copy engine");
+    if (!encode_q(&map_q, a, half) || !encode_store(&map_k, a, a.k, half) || !encode_store(&map_v, a, a.v, half))
+        return ctx->fail(LOKAL_ERR_CUDA, "tree_attn: q or a store cannot be described to the copy engine");
     const unsigned shares = static_cast<unsigned>(ctx->sm_count);
-    launch_staged(tree_attn_tc_kernel<T, HD>, shares, kTcThreads, TcShape<HD>::kBytes, s, a, map_k, map_v);
+    launch_staged(tree_attn_tc_kernel<T, HD>, shares, kTcThreads, TcShape<HD>::kBytes, s, a, map_q, map_k, map_v);
     LOKAL_CHECK_LAUNCH(ctx, "tree_attn_tc_kernel");
     launch_k(tree_join_kernel<T, kTcRows, kTcKeys>, shares - 1, 256, 0, s, a, shares);
     LOKAL_CHECK_LAUNCH(ctx, "tree_join_kernel");
@@ -571,10 +713,13 @@ int launch_tc(lokal_cuda_ctx* ctx, cudaStream_t s, const TreeArgs& a) {
 
 }  // namespace
 
+unsigned tree_tc_block(const TreeArgs& a) { return kTcRows / a.group * a.group; }
+
 size_t tree_tc_rows(const lokal_cuda_ctx* ctx) { return static_cast<size_t>(ctx->sm_count) * 2 * kTcRows; }
 
+// Rows the copy engine can take (16-byte grid), and a scale that does not turn a maximum into a minimum.
 bool tree_tc_takes(const TreeArgs& a, int dtype, int kv_dtype) {
-    return dtype == kv_dtype && dtype != LOKAL_F32 && (a.head_dim == 64 || a.head_dim == 128) && a.row_bytes % 16 == 0 && aligned_to(a.k, 16) &&
+    return dtype == kv_dtype && dtype != LOKAL_F32 && (a.head_dim == 64 || a.head_dim == 128) && a.group <= kTcRows && a.scale_log2 >= 0.0f && a.row_bytes % 16 == 0 && aligned_to(a.k, 16) &&
            aligned_to(a.v, 16) && aligned_to(a.q, 16) && aligned_to(a.out, 16) && a.q_stride % 8 == 0 && a.out_stride % 8 == 0;
 }
 
