@@ -405,6 +405,7 @@ int lokal_cuda_tree_attn(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const lokal_k
     a.wait_limit = static_cast<unsigned>(lokal::tune_env("LOKAL_CUDA_WAIT_LIMIT", lokal::kWaitLimit));
     cudaStream_t st = static_cast<cudaStream_t>(s);
     const bool tc = lokal::tree_tc_takes(a, dtype, kv_dtype);
+    a.out_vec32 = lokal::aligned_to(out, 32) && out_row_stride * es % 32 == 0;
     a.block_rows = tc ? lokal::tree_tc_block(a) : lokal::kAnyRows;
     a.part_ml = static_cast<float2*>(workspace);
     a.part_o = reinterpret_cast<float*>(a.part_ml + (tc ? lokal::tree_tc_rows(ctx) : lokal::any_rows(ctx, head_dim)));

@@ -24,13 +24,14 @@ struct TreeArgs {
     const int32_t* table;
     const int32_t* lens;
     unsigned* err_word;
-    float* part_o;    // [CTA][2][R][head_dim]
+    float* part_o;    // [CTA][2][R][head_dim] (tensor-core kernel: [CTA][2][head_dim][R])
     float2* part_ml;  // [CTA][2][R]: maximum (in units of log 2) and sum
     unsigned long long q_stride, out_stride, row_bytes;
     unsigned n_seqs, rows, mask_words, n_q_heads, n_kv_heads, group, head_dim;
     unsigned page_rows, page_shift, n_pages, n_slots, max_pages;
     unsigned block_rows;  // query rows of a block: at most R
     unsigned wait_limit;
+    int out_vec32;        // rows of out start on 32-byte boundaries
     float scale_log2;  // scale * log2(e): the exponentials are powers of two
 };
 
@@ -155,22 +156,32 @@ struct TreeUnit {
     unsigned piece;   // 0 if the block is the CTA's first, else 1
 };
 
-// Steps through the tiles [at, hi) of a CTA. Every role of a CTA walks for itself.
+// Steps through the tiles [at, hi) of a CTA. Every role of a CTA walks for itself. `known` (shared memory, or NULL) holds
+// the first kTreeKnown sequences of the walk: while the copies of K and V fill the memory's queues, a load takes four
+// microseconds, and the two that a sequence needs depend on one another.
+constexpr unsigned kTreeKnown = 30;  // what is left of a CTA's shared memory
 template <int KT>
 struct TreeWalk {
-    unsigned at, hi, lo, base, cur_tiles, seq;
+    unsigned at, hi, lo, base, cur_tiles, seq, first;
+    const int4* known;
     TreeSeq cur;
-    __device__ void start(const TreeArgs& a, const TreePlace& p, unsigned from, unsigned to) {
+    __device__ void start(const TreeArgs& a, const TreePlace& p, unsigned from, unsigned to, const int4* known_ = nullptr) {
         lo = at = from;
         hi = to;
         base = p.base;
-        seq = p.seq;
+        seq = first = p.seq;
+        known = known_;
         cur = TreeSeq{0u, 0u, 0, 0, 0u};
         cur_tiles = 0;
         if (at < hi) load(a);
     }
     __device__ void load(const TreeArgs& a) {
-        cur = tree_seq(a, seq, false);
+        if (known && seq - first < kTreeKnown) {
+            const int4 k = known[seq - first];
+            cur = TreeSeq{static_cast<unsigned>(k.x), static_cast<unsigned>(k.y), k.z - k.y, k.z, static_cast<unsigned>(k.w)};
+        } else {
+            cur = tree_seq(a, seq, false);
+        }
         cur_tiles = static_cast<unsigned>(tree_tiles<KT>(a, cur));
     }
     __device__ bool next(const TreeArgs& a, TreeUnit& u) {
@@ -222,6 +233,19 @@ __device__ __forceinline__ unsigned tree_visible(const TreeArgs& a, const TreeSe
         bits = static_cast<unsigned>(w);
     }
     return in & bits;
+}
+
+// The same 32 bits from the first two words of the row's mask, for sequences of up to 128 drafted rows.
+__device__ __forceinline__ unsigned tree_visible2(const TreeArgs& a, const TreeSeq& q, unsigned node, int pos0, unsigned long long w0, unsigned long long w1) {
+    if (!a.mask) return tree_visible(a, q, node, pos0);
+    const int left = q.len - pos0, u0 = pos0 - q.ctx;
+    if (left <= 0) return 0u;
+    const unsigned in = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
+    if (u0 + 31 < 0) return in;
+    if (u0 < 0) return in & ((static_cast<unsigned>(w0) << -u0) | ((1u << -u0) - 1u));
+    const unsigned sh = static_cast<unsigned>(u0) & 63u;
+    const unsigned long long lo = u0 < 64 ? w0 : u0 < 128 ? w1 : 0ull, hi = u0 < 64 ? w1 : 0ull;
+    return in & static_cast<unsigned>((lo >> sh) | (sh ? hi << (64u - sh) : 0ull));
 }
 
 // Cache row of a position. A page that is not there is read as page 0 and reported: nothing outside the pool is touched.

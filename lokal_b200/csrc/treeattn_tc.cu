@@ -29,22 +29,27 @@
 namespace lokal {
 namespace {
 
+constexpr unsigned kMaxShares = 512;  // CTAs of the attention kernel, one per SM: more are not used
 constexpr int kTcRows = 128, kTcKeys = 128, kTcThreads = 384;
+constexpr unsigned kSoftmaxThreads = 256;
 
 template <int HD>
 struct TcShape {
     static constexpr int kSubs = HD / 64;             // 64-column panels of 128 bytes
     static constexpr unsigned kPanel = 128 * 128;     // bytes of a panel of 128 rows
     static constexpr unsigned kTile = kSubs * kPanel; // bytes of a K or V tile, and of Q
-    static constexpr unsigned kSlots = HD == 128 ? 6 : 13;  // K and V tiles in the ring: 192 / 208 KB beside Q
+    static constexpr unsigned kSlots = HD == 128 ? 5 : 10;  // K and V tiles in the ring: 160 KB beside two Q tiles
     static constexpr unsigned kScores = HD == 128 ? 2 : 3;  // S tiles in TMEM: 128 columns each, beside two accumulators of HD
     static constexpr unsigned kAhead = kScores - 1;         // tiles whose scores are computed before a tile's output product
-    static constexpr unsigned kRing = kTile;
+    static constexpr unsigned kUnits = 8;  // blocks that the scores may be ahead of the last one written out: four at most
+    static constexpr unsigned kRing = 2 * kTile;
     static constexpr unsigned kMl = kRing + kSlots * kTile;  // float2[2][128]
     static constexpr unsigned kBars = kMl + 2 * 128 * 8;     // mbarriers
-    static constexpr unsigned kNumBars = 2 * kSlots + 3 * kScores + 3;
+    static constexpr unsigned kNumBars = 2 * kSlots + 3 * kScores + 5 + kUnits + 1;
     static constexpr unsigned kMisc = kBars + (kNumBars + 1) / 2 * 16;  // TMEM address, flags
-    static constexpr unsigned kBytes = kMisc + 32;
+    static constexpr unsigned kKnown = kMisc + 32;                      // sequences of the walk
+    static constexpr unsigned kUnit = kKnown + kTreeKnown * 16;         // blocks, for the softmax groups
+    static constexpr unsigned kBytes = kUnit + kUnits * 32;
     static_assert(kBytes <= 227 * 1024, "a CTA's shared memory");
     static_assert(kScores * 128 + 2 * HD <= 512, "TMEM columns");
 };
@@ -152,12 +157,16 @@ __device__ __forceinline__ constexpr uint32_t tc_idesc(unsigned fmt, unsigned n,
 }
 
 __device__ __forceinline__ void mbar_arrive(uint32_t mbar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(mbar) : "memory"); }
+__device__ __forceinline__ bool mbar_is_done(uint32_t mbar, unsigned parity) {  // a look, without waiting
+    unsigned yes;
+    asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(yes) : "r"(mbar), "r"(parity) : "memory");
+    return yes != 0;
+}
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t mbar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
                  "l"(map), "r"(x), "r"(y), "r"(mbar)
                  : "memory");
 }
-__device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {  // 2 steps of error, 0 for results below the smallest normal value
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -189,6 +198,8 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
                  : "memory");
 }
 
+__device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+
 // A wait that gives up: after `limit` polls, or when another role of the CTA has.
 __device__ __forceinline__ bool tc_wait(uint32_t mbar, unsigned parity, unsigned limit, volatile int* gave_up) {
     if (mbar_try_wait(mbar, parity)) return true;
@@ -200,19 +211,45 @@ __device__ __forceinline__ bool tc_wait(uint32_t mbar, unsigned parity, unsigned
     return false;
 }
 
+// Sixteen 16-bit values of a row: a whole 32-byte sector where the rows allow it.
+__device__ __forceinline__ void st_row16(void* p, const uint32_t (&h)[8], bool vec32) {
+    if (vec32) {
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), TC_W4(h, 0), TC_W4(h, 4) : "memory");
+    } else {
+        static_cast<uint4*>(p)[0] = make_uint4(h[0], h[1], h[2], h[3]);
+        static_cast<uint4*>(p)[1] = make_uint4(h[4], h[5], h[6], h[7]);
+    }
+}
+
+// Pieces are kept by column, the rows of a column side by side: the 32 threads that hold 32 rows of an accumulator write
+// 128 bytes at a time (by row they wrote 16 bytes each to 32 lines: 8,000 clocks for a piece of 128 x 128, now 2,000).
+__device__ __forceinline__ size_t piece_at(size_t piece, unsigned head_dim, unsigned col, unsigned row) {
+    return (piece * head_dim + col) * kTcRows + row;
+}
+
+// A block as the softmax groups need it, in shared memory; n == 0 ends the walk.
+struct __align__(16) TcUnit {
+    unsigned row0, len, block, kv_head;
+    unsigned k0, n;         // key tiles k0 .. k0 + n
+    unsigned drafted;       // drafted rows of the sequence
+    unsigned slot_piece;    // slot * 4 + whole * 2 + piece
+    __device__ int ctx() const { return static_cast<int>(len - drafted); }
+};
+
 // V rows that hold an infinity or a NaN and belong to drafted rows were cleared for the product, because rows that do not
 // see them would get 0 * inf. What they add to the rows that do see them is added here, to the stored result: rare, and
 // slow (a dot product per row and value).
 template <typename T, int HD>
-__device__ __noinline__ void add_bad_values(const TreeArgs& a, const TreeUnit& u, unsigned node, unsigned head, float m, float l, T* out, float* piece,
+__device__ __noinline__ void add_bad_values(const TreeArgs& a, const TcUnit* unit, unsigned node, unsigned head, float m, float l, T* out, float* piece,
                                             unsigned c0, unsigned c1) {
-    const int first = max(u.seq.ctx, static_cast<int>(u.k0) * kTcKeys), last = min(u.seq.len, static_cast<int>(u.k1) * kTcKeys);
-    const T* q = static_cast<const T*>(a.q) + static_cast<size_t>(u.seq.row0 + node) * a.q_stride + static_cast<size_t>(head) * HD;
+    const TreeSeq seq{unit->row0, unit->drafted, unit->ctx(), static_cast<int>(unit->len), unit->slot_piece >> 2};
+    const int first = max(seq.ctx, static_cast<int>(unit->k0) * kTcKeys), last = min(seq.len, static_cast<int>(unit->k0 + unit->n) * kTcKeys);
+    const T* q = static_cast<const T*>(a.q) + static_cast<size_t>(seq.row0 + node) * a.q_stride + static_cast<size_t>(head) * HD;
     for (int pos = first; pos < last; pos++) {
-        if (!(tree_visible(a, u.seq, node, pos) & 1u)) continue;
-        const size_t row = (static_cast<size_t>(tree_page(a, u.seq.slot, static_cast<unsigned>(pos) >> a.page_shift)) << a.page_shift) +
+        if (!(tree_visible(a, seq, node, pos) & 1u)) continue;
+        const size_t row = (static_cast<size_t>(tree_page(a, seq.slot, static_cast<unsigned>(pos) >> a.page_shift)) << a.page_shift) +
                            (static_cast<unsigned>(pos) & (a.page_rows - 1));
-        const size_t off = row * a.row_bytes + static_cast<size_t>(u.kv_head) * HD * 2;
+        const size_t off = row * a.row_bytes + static_cast<size_t>(unit->kv_head) * HD * 2;
         const T* v = reinterpret_cast<const T*>(a.v + off);
         const T* k = reinterpret_cast<const T*>(a.k + off);
         float p = 0.0f;
@@ -226,7 +263,7 @@ __device__ __noinline__ void add_bad_values(const TreeArgs& a, const TreeUnit& u
                 p = exp2f(fmaf(s, a.scale_log2, -m));
                 have = true;
             }
-            if (piece) piece[c] += p * x;
+            if (piece) piece[static_cast<size_t>(c) * kTcRows] += p * x;
             else out[c] = from_f32<T>(to_f32<T>(out[c]) + p * x / l);
         }
     }
@@ -246,7 +283,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const auto sfull = [&](unsigned b) { return bars + (2 * S::kSlots + b) * 8; };                  // scores are there
     const auto pready = [&](unsigned b) { return bars + (2 * S::kSlots + S::kScores + b) * 8; };    // weights are there
     const auto sfree = [&](unsigned b) { return bars + (2 * S::kSlots + 2 * S::kScores + b) * 8; };  // weights have been used
-    const uint32_t qfull = bars + (2 * S::kSlots + 3 * S::kScores) * 8, qfree = qfull + 8, udone = qfull + 16;  // udone: the last product of a block
+    const uint32_t qfull = bars + (2 * S::kSlots + 3 * S::kScores) * 8, qfree = qfull + 16, udone = qfull + 32;  // Q tiles 0 and 1 each; the last product of a block
+    const uint32_t ufull = udone + 8, fbar = ufull + 8 * S::kUnits;  // a block is described; the softmax groups meet
     volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(tc_smem + S::kMisc);  // [0] TMEM, [1] a wait gave up, [2..5] bad values, by block
     volatile int* gave_up = reinterpret_cast<volatile int*>(misc + 1);
     float2* ml = reinterpret_cast<float2*>(tc_smem + S::kMl);
@@ -259,13 +297,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 mbar_init(pready(b), 128);
                 mbar_init(sfree(b), 1);
             }
-            mbar_init(qfull, 1);
-            mbar_init(qfree, 1);
+            for (unsigned b = 0; b < 2; b++) {
+                mbar_init(qfull + 8 * b, 1);
+                mbar_init(qfree + 8 * b, 1);
+            }
             mbar_init(udone, 1);
+            for (unsigned i = 0; i < S::kUnits; i++) mbar_init(ufull + 8 * i, 1);
+            mbar_init(fbar, kSoftmaxThreads);
             mbar_init_fence();
             for (int i = 1; i < 6; i++) misc[i] = 0;
         }
     }
+    if (warp == 9 && lane < 3) tma_prefetch(lane == 0 ? &map_q : lane == 1 ? &map_k : &map_v);
     pdl_sync();
     // the ring is not in use yet: its first bytes hold the sums of the walk
     const unsigned shares = gridDim.x;
@@ -273,6 +316,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const TreeShares s(total, shares);
         return blockIdx.x < s.g ? s.first(blockIdx.x) : total;
     });
+    int4* known = reinterpret_cast<int4*>(tc_smem + S::kKnown);
+    if (warp == 10 && lane < kTreeKnown && place.seq + lane < a.n_seqs) {
+        const TreeSeq q = tree_seq(a, place.seq + lane, false);
+        known[lane] = make_int4(static_cast<int>(q.row0), static_cast<int>(q.n), q.len, static_cast<int>(q.slot));
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -280,7 +328,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const TreeShares share(place.total, shares);
     bool ok = place.seq < a.n_seqs;
     TreeWalk<kTcKeys> walk;
-    walk.start(a, place, ok ? share.first(blockIdx.x) : 0u, ok ? share.first(blockIdx.x + 1) : 0u);
+    walk.start(a, place, ok ? share.first(blockIdx.x) : 0u, ok ? share.first(blockIdx.x + 1) : 0u, known);
     TreeUnit u;
 
     if (warp == 8 || warp == 11) {
@@ -291,26 +339,46 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         RingAt<HD> at;
         bool reused = false;               // the ring has been round once
         unsigned units = 0, issued = 0, parity = 0;  // blocks; by slot: whether it was filled, and in which round
+        // query rows: a walk of its own, a block ahead
+        TreeWalk<kTcKeys> q_walk = walk;
+        TreeUnit q_unit;
+        unsigned q_block = 0, q_blocks = 0;  // the next, and how many have been asked for
+        bool q_more = !is_k && ok && q_walk.next(a, q_unit);
+        const auto put_q = [&](bool must) {
+            const unsigned b = q_block & 1u;
+            if (!q_more) {
+                q_block = 0xffffffffu;
+                return;
+            }
+            if (q_block >= 2) {
+                const unsigned phase = ((q_block >> 1) - 1) & 1u;
+                if (must) ok = __all_sync(0xffffffffu, tc_wait(qfree + 8 * b, phase, a.wait_limit, gave_up));
+                else if (!__all_sync(0xffffffffu, mbar_is_done(qfree + 8 * b, phase))) return;
+                if (!ok) return;
+            }
+            if (lane == 0) {
+                const unsigned nodes = kTcRows / a.group;
+                mbar_expect_tx(qfull + 8 * b, nodes * a.group * 128 * S::kSubs);
+#pragma unroll
+                for (int c = 0; c < S::kSubs; c++)
+                    tma_load_3d(smem + b * S::kTile + c * S::kPanel, &map_q, c * 64, static_cast<int>(q_unit.kv_head * a.group), static_cast<int>(q_unit.seq.row0 + q_unit.block * nodes),
+                                qfull + 8 * b);
+            }
+            __syncwarp();
+            q_block++;
+            q_blocks++;
+            q_more = q_walk.next(a, q_unit);
+        };
         while (ok && walk.next(a, u)) {
             const unsigned n = u.k1 - u.k0;
-            // lane b names the page of box b of a tile; the next tile's page is on its way while this tile is copied
-            const auto row_of = [&](unsigned i) -> int {
-                const unsigned pos = (u.k0 + i) * kTcKeys + lane * box_rows;
-                if (i >= n || lane * box_rows >= kTcKeys || pos >= static_cast<unsigned>(u.seq.len)) return 0;
-                return static_cast<int>((tree_page(a, u.seq.slot, pos >> a.page_shift) << a.page_shift) + (pos & (a.page_rows - 1)));
-            };
-            int y = row_of(0);
+            // The block's pages, 32 at a time, a lane each, the next 32 on their way (pages to a tile divide 32, so no tile
+            // lies across two batches).
+            const unsigned first_page = u.k0 * kTcKeys >> a.page_shift, last_page = (min(u.k1 * kTcKeys, static_cast<unsigned>(u.seq.len)) - 1) >> a.page_shift;
+            const auto pages_at = [&](unsigned p) { return p + lane <= last_page ? tree_page(a, u.seq.slot, p + lane) : 0u; };
+            unsigned page0 = first_page, pages = pages_at(first_page), pages_next = pages_at(first_page + 32);
             if (!is_k) {
-                if (units) ok = __all_sync(0xffffffffu, tc_wait(qfree, (units - 1) & 1u, a.wait_limit, gave_up));
-                if (!ok) break;
-                if (lane == 0) {
-                    const unsigned nodes = kTcRows / a.group;
-                    mbar_expect_tx(qfull, nodes * a.group * 128 * S::kSubs);
-#pragma unroll
-                    for (int c = 0; c < S::kSubs; c++)
-                        tma_load_3d(smem + c * S::kPanel, &map_q, c * 64, static_cast<int>(u.kv_head * a.group), static_cast<int>(u.seq.row0 + u.block * nodes), qfull);
-                }
-                __syncwarp();
+                // this block's query rows unless they are on their way, and the next block's as soon as their tile is free
+                while (ok && q_block <= units) put_q(true);
                 units++;
             }
             unsigned behind = is_k ? 0u : v_place<HD>(0, n);
@@ -324,6 +392,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const unsigned boxes = (min(left, static_cast<unsigned>(kTcKeys)) + box_rows - 1) / box_rows;
                 issued |= 1u << at.slot;
                 parity = (parity & ~(1u << at.slot)) | (at.round << at.slot);
+                const unsigned pos = (u.k0 + i) * kTcKeys, page = pos >> a.page_shift;
+                if (page - page0 >= 32) {
+                    page0 += 32;
+                    pages = pages_next;
+                    pages_next = pages_at(page0 + 32);
+                }
+                const unsigned mine = __shfl_sync(0xffffffffu, pages, min(page - page0 + lane, 31u));
+                const int y = static_cast<int>((mine << a.page_shift) + (pos & (a.page_rows - 1)));
                 if (lane == 0) mbar_expect_tx(full(at.slot), boxes * box_rows * 128 * S::kSubs);
                 __syncwarp();
                 if (lane < boxes) {
@@ -331,7 +407,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                     for (int c = 0; c < S::kSubs; c++) tma_load_2d(to + c * S::kPanel, map, x + c * 64, y, full(at.slot));
                 }
-                y = row_of(i + 1);
+                if (!is_k && q_block <= units) put_q(false);
                 const unsigned next = i + 1 == n ? 2 * n : is_k ? i + 1 + (i + 1 > S::kAhead ? i + 1 - S::kAhead : 0u) : v_place<HD>(i + 1, n);
                 reused |= at.slot + (next - behind) >= S::kSlots;
                 at.add(next - behind);
@@ -342,6 +418,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // what is in flight lands before the CTA gives its memory back
             for (unsigned slot = 0; slot < S::kSlots; slot++)
                 if ((issued >> slot) & 1u) mbar_wait_bounded(full(slot), (parity >> slot) & 1u, a.wait_limit);
+            if (!is_k) {
+                for (unsigned q = q_blocks > 2 ? q_blocks - 2 : 0u; q < q_blocks; q++) mbar_wait_bounded(qfull + 8 * (q & 1u), (q >> 1) & 1u, a.wait_limit);
+            }
         }
     } else if (warp == 9) {
         // ---- S = Q K^T ----
@@ -350,24 +429,33 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         RingAt<HD> at;                     // of the next K tile
         unsigned b = 0, b_round = 0, t = 0, units = 0;  // S tile, key tiles, blocks
         const auto wait = [&](uint32_t bar, unsigned parity) { ok = ok && __all_sync(0xffffffffu, tc_wait(bar, parity, a.wait_limit, gave_up)); };
+        TcUnit* described = reinterpret_cast<TcUnit*>(tc_smem + S::kUnit);
+        const auto publish = [&](unsigned n) {  // block `units`, to the softmax groups
+            if (lane == 0) {
+                described[units % S::kUnits] = TcUnit{u.seq.row0, static_cast<unsigned>(u.seq.len), u.block, u.kv_head, u.k0, n, u.seq.n, u.seq.slot * 4 + (u.whole ? 2u : 0u) + u.piece};
+                mbar_arrive(ufull + 8 * (units % S::kUnits));
+            }
+            __syncwarp();
+        };
         while (ok && walk.next(a, u)) {
-            const unsigned n = u.k1 - u.k0;
-            wait(qfull, units & 1u);
+            const unsigned n = u.k1 - u.k0, qb = units & 1u;
+            publish(n);
+            wait(qfull + 8 * qb, (units >> 1) & 1u);
             for (unsigned i = 0; ok && i < n; i++) {
                 wait(full(at.slot), at.round);
                 if (t >= S::kScores) wait(sfree(b), b_round ^ 1u);  // the weights that these scores overwrite have been used
                 if (!ok) break;
                 tc_fence_after();
                 if (tc_elect()) {
-                    const uint64_t kd = k_desc + at.slot * (S::kTile >> 4);
+                    const uint64_t qd = q_desc + qb * (S::kTile >> 4), kd = k_desc + at.slot * (S::kTile >> 4);
 #pragma unroll
                     for (int k = 0; k < HD / 16; k++) {
                         const unsigned off = ((k / 4) * S::kPanel + (k % 4) * 32) >> 4;
-                        tc_mma_ss(tmem + b * 128, q_desc + off, kd + off, idesc, k != 0);
+                        tc_mma_ss(tmem + b * 128, qd + off, kd + off, idesc, k != 0);
                     }
                     tc_commit(sfull(b));
                     tc_commit(empty(at.slot));
-                    if (i == n - 1) tc_commit(qfree);
+                    if (i == n - 1) tc_commit(qfree + 8 * qb);
                 }
                 __syncwarp();
                 if (++b == S::kScores) {
@@ -379,6 +467,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             units++;
         }
+        if (ok) publish(0);
         if (!ok && place.seq < a.n_seqs) {
             // the products in flight end before TMEM is given back
             if (t) mbar_wait_bounded(sfull((t - 1) % S::kScores), ((t - 1) / S::kScores) & 1u, a.wait_limit);
@@ -434,19 +523,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t lanes = (warp & 3u) << 21;  // the warp's 32 lanes of TMEM
         const uint32_t o_at = tmem + S::kScores * 128 + lanes;
         const float scale = a.scale_log2;
-        unsigned t = 0, seq0 = 0, units = 0;  // key tiles, ring tiles and blocks before the block
-        // the block that is done but not yet written
-        TreeUnit last{};
+        unsigned t = 0, units = 0;  // key tiles and blocks before the block (a key tile is two of the ring's)
+        const TcUnit* described = reinterpret_cast<const TcUnit*>(tc_smem + S::kUnit);
+        // of the block before this one, which may not have been written yet
         float last_m = 0.0f, last_l = 0.0f;
         bool pending = false;
+        // The two groups meet, twice for every block. (A wait that can give up, not a hardware barrier: were one group to
+        // give up on something else, the other would stand there for good.)
+        const auto meet = [&](unsigned phase) {
+            mbar_arrive(fbar);
+            ok = __all_sync(0xffffffffu, tc_wait(fbar, phase, a.wait_limit, gave_up)) && ok;
+        };
         // The two streams of a block are put together and written out.
         const auto finish = [&] {
             const unsigned which = units - 1;  // the block's number
-            const unsigned flat0 = last.block * a.block_rows, m_rows = min(a.block_rows, last.seq.n * a.group - flat0);
+            const TcUnit* last = described + which % S::kUnits;
+            const bool whole = (last->slot_piece & 2u) != 0;
+            const unsigned flat0 = last->block * a.block_rows, m_rows = min(a.block_rows, last->drafted * a.group - flat0);
             ok = __all_sync(0xffffffffu, ok && tc_wait(udone, which & 1u, a.wait_limit, gave_up));
             tc_fence_after();
             ml[w * 128 + row] = make_float2(last_m, last_l);
-            bar_softmax();
+            meet(0);
             const bool fix = misc[2 + (which & 3u)] != 0;
             if (tid == 0) misc[2 + ((which + 2) & 3u)] = 0;  // read two blocks ago, written again only behind the barrier below
             const float2 other = ml[(w ^ 1u) * 128 + row];
@@ -456,10 +553,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const float total = (last_l == 0.0f ? 0.0f : last_l * f_own) + (other.y == 0.0f ? 0.0f : other.y * f_other);
             const float inv = total == 0.0f ? 0.0f : 1.0f / total;
             if ((warp & 3u) * 32 < m_rows) {
-                const unsigned flat = flat0 + min(row, m_rows - 1), node = flat / a.group, head = last.kv_head * a.group + flat % a.group;
-                T* out = static_cast<T*>(a.out) + static_cast<size_t>(last.seq.row0 + node) * a.out_stride + static_cast<size_t>(head) * HD;
-                const size_t piece = (static_cast<size_t>(blockIdx.x) * 2 + last.piece) * kTcRows + row;
-                float* po = a.part_o + piece * HD;
+                const unsigned flat = flat0 + min(row, m_rows - 1), node = flat / a.group, head = last->kv_head * a.group + flat % a.group;
+                T* out = static_cast<T*>(a.out) + static_cast<size_t>(last->row0 + node) * a.out_stride + static_cast<size_t>(head) * HD;
+                float* po = a.part_o + piece_at(blockIdx.x * 2 + (last->slot_piece & 1u), HD, 0, row);
                 const unsigned c0 = w * (HD / 2);
 #pragma unroll
                 for (int j = 0; j < HD / 64; j++) {
@@ -473,26 +569,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int i = 0; i < 32; i++)
                         o[i] = fmaf(last_l == 0.0f ? 0.0f : __uint_as_float(x[i]), f_own, other.y == 0.0f ? 0.0f : __uint_as_float(y[i]) * f_other);
                     if (row < m_rows) {
-                        if (last.whole) {
+                        if (whole) {
 #pragma unroll
-                            for (int i = 0; i < 32; i += 8)
-                                *reinterpret_cast<uint4*>(out + c0 + 32 * j + i) =
-                                    make_uint4(pack2<T>(o[i] * inv, o[i + 1] * inv), pack2<T>(o[i + 2] * inv, o[i + 3] * inv),
-                                               pack2<T>(o[i + 4] * inv, o[i + 5] * inv), pack2<T>(o[i + 6] * inv, o[i + 7] * inv));
+                            for (int i = 0; i < 32; i += 16) {
+                                uint32_t h[8];
+#pragma unroll
+                                for (int k = 0; k < 8; k++) h[k] = pack2<T>(o[i + 2 * k] * inv, o[i + 2 * k + 1] * inv);
+                                st_row16(out + c0 + 32 * j + i, h, a.out_vec32);
+                            }
                         } else {
 #pragma unroll
-                            for (int i = 0; i < 32; i += 4)
-                                *reinterpret_cast<float4*>(po + c0 + 32 * j + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                            for (int i = 0; i < 32; i++) po[static_cast<size_t>(c0 + 32 * j + i) * kTcRows] = o[i];
                         }
                     }
                 }
                 if (row < m_rows) {
-                    if (!last.whole && w == 0) a.part_ml[piece] = make_float2(top, total);
-                    if (fix && total != 0.0f) add_bad_values<T, HD>(a, last, node, head, ref, total, out, last.whole ? nullptr : po, c0, c0 + HD / 2);
+                    if (!whole && w == 0) a.part_ml[(blockIdx.x * 2 + (last->slot_piece & 1u)) * kTcRows + row] = make_float2(top, total);
+                    if (fix && total != 0.0f) add_bad_values<T, HD>(a, last, node, head, ref, total, out, whole ? nullptr : po, c0, c0 + HD / 2);
                 }
             }
             tc_fence_before();
-            bar_softmax();  // the accumulators may be written again
+            meet(1);  // the accumulators may be written again
             pending = false;
         };
         float m = 0.0f, l = 0.0f;  // of the block, for this stream
@@ -570,12 +667,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         };
         // V rows behind the last position are cleared (they may hold anything, and 0 * NaN is NaN); so are drafted ones with an
         // infinity or a NaN, which rows that do not see them must not get: add_bad_values.
-        const auto clear_v = [&](unsigned i, unsigned n, int pos0) {
-            const unsigned at = seq0 + v_place<HD>(i, n), slot = at % S::kSlots;
+        const auto clear_v = [&](unsigned i, unsigned n, int valid, int drafted) {
+            const unsigned at = 2 * t + v_place<HD>(i, n), slot = at % S::kSlots;
             ok = __all_sync(0xffffffffu, ok && tc_wait(full(slot), (at / S::kSlots) & 1u, a.wait_limit, gave_up));
             if (!ok) return;
             unsigned char* v_at = tc_smem + S::kRing + slot * S::kTile;
-            const int valid = min(kTcKeys, u.seq.len - pos0), drafted = max(0, u.seq.ctx - pos0);
             const unsigned pieces = S::kSubs * 8;  // of 16 bytes, to a row
             for (unsigned e = row; e < (kTcKeys - valid) * pieces; e += 128) {
                 const unsigned r = valid + e / pieces, c = e % pieces;
@@ -602,12 +698,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             proxy_fence();
         };
-        // Whether or not a wait has given up: the two groups meet at the barriers of every block.
-        for (;;) {
-            const bool more = walk.next(a, u);
-            if (!more && !pending) break;
-            const unsigned n = more ? u.k1 - u.k0 : 0u;
-            const unsigned flat0 = u.block * a.block_rows, m_rows = min(a.block_rows, u.seq.n * a.group - flat0);
+        if (place.seq >= a.n_seqs) ok = false;
+        while (ok) {
+            ok = __all_sync(0xffffffffu, tc_wait(ufull + 8 * (units % S::kUnits), (units / S::kUnits) & 1u, a.wait_limit, gave_up));
+            if (!ok) break;
+            const TcUnit* now = described + units % S::kUnits;
+            const unsigned n = now->n;
+            if (n == 0 && !pending) break;
+            const unsigned flat0 = now->block * a.block_rows, m_rows = min(a.block_rows, now->drafted * a.group - flat0);
+            const unsigned node = (flat0 + min(row, m_rows - 1)) / a.group;
+            const int pos_first = static_cast<int>(now->k0) * kTcKeys, ctx = now->ctx();
+            const bool busy = (warp & 3u) * 32 < m_rows;  // some row of the warp is there
+            // the row's mask is asked for now and needed with the last tiles
+            unsigned long long w0 = 0, w1 = 0;
+            if (n && a.mask && pos_first + static_cast<int>(n) * kTcKeys > ctx) {
+                const unsigned long long* mask = a.mask + static_cast<size_t>(now->row0 + node) * a.mask_words;
+                w0 = mask[0];
+                if (a.mask_words > 1) w1 = mask[1];
+            }
             m = -INFINITY;
             l = 0.0f;
             begun = false;
@@ -618,19 +726,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (has) ok = has = __all_sync(0xffffffffu, tc_wait(sfull(b), ((t + i) / S::kScores) & 1u, a.wait_limit, gave_up));
                 if (has) {
                     tc_fence_after();
-                    const int pos0 = static_cast<int>(u.k0 + i) * kTcKeys;
-                    const bool busy = (warp & 3u) * 32 < m_rows;  // some row of the warp is there
+                    const int pos0 = pos_first + static_cast<int>(i) * kTcKeys;
                     unsigned bits[4];
-                    if (pos0 + kTcKeys <= u.seq.ctx) {
+                    if (pos0 + kTcKeys <= ctx) {
                         if (busy) weigh(std::false_type{}, tmem + b * 128 + lanes, i, bits);
                     } else {
+                        const int len = static_cast<int>(now->len);
                         if (busy) {
-                            const unsigned node = (flat0 + min(row, m_rows - 1)) / a.group;
+                            const TreeSeq seq{now->row0, now->drafted, ctx, len, 0u};
 #pragma unroll
-                            for (int j = 0; j < 4; j++) bits[j] = tree_visible(a, u.seq, node, pos0 + 32 * j);
+                            for (int j = 0; j < 4; j++)
+                                bits[j] = seq.n <= 128 ? tree_visible2(a, seq, node, pos0 + 32 * j, w0, w1) : tree_visible(a, seq, node, pos0 + 32 * j);
                             weigh(std::true_type{}, tmem + b * 128 + lanes, i, bits);
                         }
-                        clear_v(i, n, pos0);
+                        clear_v(i, n, min(kTcKeys, len - pos0), max(0, ctx - pos0));
                     }
                     begun = true;
                 }
@@ -641,13 +750,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 i += 2;
             } while (i < n);
-            if (!more) break;
-            last = u;
+            if (n == 0) break;
             last_m = m;
             last_l = l;
             pending = true;
             t += n;
-            seq0 += 2 * n;
             units++;
         }
     }
@@ -656,6 +763,83 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc_fence_after();
     if (tid == 0 && *gave_up) atomicOr(a.err_word, kErrTimeout);
     if (warp == 8) tc_dealloc(tmem, 512);
+}
+
+// Joins the pieces of blocks that several CTAs share. CTA c stands at the border between shares c and c + 1; the CTAs at
+// the borders inside one block (eight CTAs to a border) divide it among them in parts of 8 rows by 32 columns, a thread to
+// each value. The pieces' weights are worked out once for the rows at hand; eight pieces are in flight at a time.
+template <typename T>
+__global__ void __launch_bounds__(256) tree_join_tc_kernel(const TreeArgs a, unsigned shares) {
+    pdl_sync();
+    __shared__ unsigned long long sh[2 * 8 + 4];
+    __shared__ float weight[kMaxShares + 1][8];
+    __shared__ float row_sum[8];
+    const unsigned c = blockIdx.x + 1;
+    const TreePlace p = tree_locate<kTcKeys, 256>(a, sh, false, [&](unsigned total) {
+        const TreeShares s(total, shares);
+        return c < s.g ? s.first(c) : total;
+    });
+    if (p.seq >= a.n_seqs) return;
+    const TreeShares s(p.total, shares);
+    const unsigned border = s.first(c);
+    const TreeSeq q = tree_seq(a, p.seq, false);
+    const unsigned kt = (static_cast<unsigned>(q.len) + kTcKeys - 1) / kTcKeys;
+    const unsigned rows_all = q.n * a.group, blocks = (rows_all + a.block_rows - 1) / a.block_rows;
+    const unsigned unit = (border - p.base) / kt;
+    const unsigned t0 = p.base + unit * kt;
+    if (border == t0) return;
+    const unsigned first = s.owner(t0) + 1, last = s.owner(t0 + kt - 1);  // borders inside the block
+    const unsigned n_borders = last - first + 1, n_pieces = n_borders + 1;
+    const unsigned kv_head = unit / blocks, block = unit - kv_head * blocks;
+    const unsigned m_rows = min(a.block_rows, rows_all - block * a.block_rows);
+    const unsigned cols = a.head_dim / 32, parts = (m_rows + 7) / 8 * cols;
+    const unsigned mine = (c - first) * gridDim.y + blockIdx.y, of = n_borders * gridDim.y;
+    const unsigned part1 = parts * (mine + 1) / of;
+    // piece x (0 ..) is left by share first - 1 + x; only the first of them may be a CTA's second block
+    const bool second = s.first(first - 1) < t0;
+    const auto piece = [&](unsigned x) { return static_cast<size_t>(first - 1 + x) * 2 + (x == 0 && second ? 1 : 0); };
+    const unsigned r = threadIdx.x & 7u, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    unsigned rows_at = 0xffffffffu;
+    for (unsigned part = parts * mine / of; part < part1; part++) {
+        const unsigned row0 = part / cols * 8, col = part % cols * 32 + (threadIdx.x >> 3);
+        if (row0 != rows_at) {
+            // a warp takes a row: the largest maximum, then the weights and their sum
+            rows_at = row0;
+            __syncthreads();
+            const bool in = row0 + warp < m_rows;
+            float top = -INFINITY, l = 0.0f;
+            if (in)
+                for (unsigned x = lane; x < n_pieces; x += 32) top = fmaxf(top, a.part_ml[piece(x) * kTcRows + row0 + warp].x);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            for (unsigned x = lane; x < n_pieces; x += 32) {
+                float w = 0.0f;  // stays 0 where nothing of a piece was visible
+                if (in) {
+                    const float2 ml = a.part_ml[piece(x) * kTcRows + row0 + warp];
+                    if (ml.y != 0.0f) {
+                        w = ex2(ml.x - (top == -INFINITY ? 0.0f : top));
+                        l = fmaf(ml.y, w, l);
+                    }
+                }
+                weight[x][warp] = w;
+            }
+            l = warp_sum(l);
+            if (lane == 0) row_sum[warp] = l;
+            __syncthreads();
+        }
+        const unsigned row = row0 + r;
+        if (row >= m_rows) continue;
+        float acc = 0.0f;
+#pragma unroll 8
+        for (unsigned x = 0; x < n_pieces; x++) {
+            const float w = weight[x][r];
+            const float o = a.part_o[piece_at(piece(x), a.head_dim, col, row)];
+            acc = w == 0.0f ? acc : fmaf(o, w, acc);
+        }
+        const unsigned flat = block * a.block_rows + row, node = flat / a.group, head = kv_head * a.group + flat % a.group;
+        const float l = row_sum[r];
+        static_cast<T*>(a.out)[static_cast<size_t>(q.row0 + node) * a.out_stride + static_cast<size_t>(head) * a.head_dim + col] = from_f32<T>(l == 0.0f ? 0.0f : acc / l);
+    }
 }
 
 // cuTensorMapEncodeTiled by way of the runtime: the library links no driver library.
@@ -697,17 +881,19 @@ bool encode_q(CUtensorMap* map, const TreeArgs& a, bool half) {
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+unsigned tc_shares(const lokal_cuda_ctx* ctx) { return static_cast<unsigned>(ctx->sm_count) < kMaxShares ? static_cast<unsigned>(ctx->sm_count) : kMaxShares; }
+
 template <typename T, int HD>
 int launch_tc(lokal_cuda_ctx* ctx, cudaStream_t s, const TreeArgs& a) {
     CUtensorMap map_q, map_k, map_v;
     constexpr bool half = std::is_same<T, __half>::value;
     if (!encode_q(&map_q, a, half) || !encode_store(&map_k, a, a.k, half) || !encode_store(&map_v, a, a.v, half))
         return ctx->fail(LOKAL_ERR_CUDA, "tree_attn: q or a store cannot be described to the copy engine");
-    const unsigned shares = static_cast<unsigned>(ctx->sm_count);
+    const unsigned shares = tc_shares(ctx);
     launch_staged(tree_attn_tc_kernel<T, HD>, shares, kTcThreads, TcShape<HD>::kBytes, s, a, map_q, map_k, map_v);
     LOKAL_CHECK_LAUNCH(ctx, "tree_attn_tc_kernel");
-    launch_k(tree_join_kernel<T, kTcRows, kTcKeys>, shares - 1, 256, 0, s, a, shares);
-    LOKAL_CHECK_LAUNCH(ctx, "tree_join_kernel");
+    launch_k(tree_join_tc_kernel<T>, dim3(shares - 1, 8), 256, 0, s, a, shares);
+    LOKAL_CHECK_LAUNCH(ctx, "tree_join_tc_kernel");
     return LOKAL_OK;
 }
 
@@ -715,7 +901,7 @@ int launch_tc(lokal_cuda_ctx* ctx, cudaStream_t s, const TreeArgs& a) {
 
 unsigned tree_tc_block(const TreeArgs& a) { return kTcRows / a.group * a.group; }
 
-size_t tree_tc_rows(const lokal_cuda_ctx* ctx) { return static_cast<size_t>(ctx->sm_count) * 2 * kTcRows; }
+size_t tree_tc_rows(const lokal_cuda_ctx* ctx) { return static_cast<size_t>(tc_shares(ctx)) * 2 * kTcRows; }
 
 // Rows the copy engine can take (16-byte grid), and a scale that does not turn a maximum into a minimum.
 bool tree_tc_takes(const TreeArgs& a, int dtype, int kv_dtype) {
