@@ -130,6 +130,18 @@ __device__ __forceinline__ void tc_wait_ld(uint32_t (&v)[32]) {
                  :
                  : "memory");
 }
+__device__ __forceinline__ void tc_ld16(uint32_t at, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : TC_R4(v, 0), TC_R4(v, 4), TC_R4(v, 8), TC_R4(v, 12)
+        : "r"(at));
+}
+__device__ __forceinline__ void tc_wait_ld16(uint32_t (&v)[16], uint32_t (&w)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : TC_RW4(v, 0), TC_RW4(v, 4), TC_RW4(v, 8), TC_RW4(v, 12), TC_RW4(w, 0), TC_RW4(w, 4), TC_RW4(w, 8), TC_RW4(w, 12)
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tc_st32(uint32_t at, const uint32_t (&v)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
@@ -271,7 +283,7 @@ __device__ __noinline__ void add_bad_values(const TreeArgs& a, const TcUnit* uni
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1)
-    tree_attn_tc_kernel(const TreeArgs a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+    tree_attn_tc_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v) {
     using S = TcShape<HD>;
     extern __shared__ __align__(1024) unsigned char tc_smem[];
@@ -557,29 +569,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 T* out = static_cast<T*>(a.out) + static_cast<size_t>(last->row0 + node) * a.out_stride + static_cast<size_t>(head) * HD;
                 float* po = a.part_o + piece_at(blockIdx.x * 2 + (last->slot_piece & 1u), HD, 0, row);
                 const unsigned c0 = w * (HD / 2);
+#pragma unroll 1
+                for (unsigned c = c0; c < c0 + HD / 2; c += 16) {
+                    uint32_t x[16], y[16];
+                    tc_ld16(o_at + w * HD + c, x);
+                    tc_ld16(o_at + (w ^ 1u) * HD + c, y);
+                    tc_wait_ld16(x, y);
+                    float o[16];
 #pragma unroll
-                for (int j = 0; j < HD / 64; j++) {
-                    uint32_t x[32], y[32];
-                    tc_ld32(o_at + w * HD + c0 + 32 * j, x);
-                    tc_ld32(o_at + (w ^ 1u) * HD + c0 + 32 * j, y);
-                    tc_wait_ld(x);
-                    tc_wait_ld(y);
-                    float o[32];
-#pragma unroll
-                    for (int i = 0; i < 32; i++)
+                    for (int i = 0; i < 16; i++)
                         o[i] = fmaf(last_l == 0.0f ? 0.0f : __uint_as_float(x[i]), f_own, other.y == 0.0f ? 0.0f : __uint_as_float(y[i]) * f_other);
                     if (row < m_rows) {
                         if (whole) {
+                            uint32_t h[8];
 #pragma unroll
-                            for (int i = 0; i < 32; i += 16) {
-                                uint32_t h[8];
-#pragma unroll
-                                for (int k = 0; k < 8; k++) h[k] = pack2<T>(o[i + 2 * k] * inv, o[i + 2 * k + 1] * inv);
-                                st_row16(out + c0 + 32 * j + i, h, a.out_vec32);
-                            }
+                            for (int k = 0; k < 8; k++) h[k] = pack2<T>(o[2 * k] * inv, o[2 * k + 1] * inv);
+                            st_row16(out + c, h, a.out_vec32);
                         } else {
 #pragma unroll
-                            for (int i = 0; i < 32; i++) po[static_cast<size_t>(c0 + 32 * j + i) * kTcRows] = o[i];
+                            for (int i = 0; i < 16; i++) po[static_cast<size_t>(c + i) * kTcRows] = o[i];
                         }
                     }
                 }
@@ -594,10 +602,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         };
         float m = 0.0f, l = 0.0f;  // of the block, for this stream
         bool begun = false;        // a tile of this stream has gone into the accumulator
+        // Scores that the row must not see become -inf, where they lie; 32 at a time, and only where some row of the warp has any.
+        const auto hide = [&](uint32_t s_at, unsigned seen) {
+            if (!__any_sync(0xffffffffu, seen != 0xffffffffu)) return;
+            uint32_t x[32];
+            tc_ld32(s_at, x);
+            tc_wait_ld(x);
+#pragma unroll
+            for (int c = 0; c < 32; c++) x[c] = (seen >> c) & 1u ? x[c] : 0xff800000u;
+            tc_st32(s_at, x);
+        };
         // A row's 128 scores to weights, in two passes of 32 at a time with the next 32 on their way: the maximum, then the
-        // weights. MASKED: drafted rows, or the end, are in the tile.
-        const auto weigh = [&](auto masked_, uint32_t s_at, unsigned i, const unsigned (&bits)[4]) {
-            constexpr bool MASKED = decltype(masked_)::value;
+        // weights.
+        const auto weigh = [&](uint32_t s_at, unsigned i) {
             uint32_t v[2][32];
             float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             tc_ld32(s_at, v[0]);
@@ -606,15 +623,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 uint32_t(&x)[32] = v[j & 1];
                 tc_wait_ld(x);
                 tc_ld32(s_at + 32 * ((j + 1) & 3), v[(j + 1) & 1]);  // after the last, the first again
-                if (MASKED) {
 #pragma unroll
-                    for (int c = 0; c < 32; c++) tops[c & 3] = (bits[j] >> c) & 1u ? fmaxf(tops[c & 3], __uint_as_float(x[c])) : tops[c & 3];
-                } else {
+                for (int c = 0; c < 32; c += 8) {
 #pragma unroll
-                    for (int c = 0; c < 32; c += 8) {
-#pragma unroll
-                        for (int k = 0; k < 4; k++) tops[k] = fmaxf(fmaxf(tops[k], __uint_as_float(x[c + k])), __uint_as_float(x[c + k + 4]));
-                    }
+                    for (int k = 0; k < 4; k++) tops[k] = fmaxf(fmaxf(tops[k], __uint_as_float(x[c + k])), __uint_as_float(x[c + k + 4]));
                 }
             }
             float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
@@ -653,10 +665,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     float2 z = fma2(make_float2(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), scale2, ref2);
                     z.x = ex2(z.x);
                     z.y = ex2(z.y);
-                    if (MASKED) {
-                        z.x = (bits[j] >> (2 * c)) & 1u ? z.x : 0.0f;
-                        z.y = (bits[j] >> (2 * c + 1)) & 1u ? z.y : 0.0f;
-                    }
                     sum[c & 1] = add2(sum[c & 1], z);
                     p[c] = pack2<T>(z.x, z.y);
                 }
@@ -727,20 +735,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (has) {
                     tc_fence_after();
                     const int pos0 = pos_first + static_cast<int>(i) * kTcKeys;
-                    unsigned bits[4];
-                    if (pos0 + kTcKeys <= ctx) {
-                        if (busy) weigh(std::false_type{}, tmem + b * 128 + lanes, i, bits);
-                    } else {
-                        const int len = static_cast<int>(now->len);
-                        if (busy) {
+                    const uint32_t s_at = tmem + b * 128 + lanes;
+                    const bool masked = pos0 + kTcKeys > ctx;  // drafted rows, or the end, are in the tile
+                    const int len = static_cast<int>(now->len);
+                    if (busy) {
+                        if (masked) {
                             const TreeSeq seq{now->row0, now->drafted, ctx, len, 0u};
-#pragma unroll
+#pragma unroll 1
                             for (int j = 0; j < 4; j++)
-                                bits[j] = seq.n <= 128 ? tree_visible2(a, seq, node, pos0 + 32 * j, w0, w1) : tree_visible(a, seq, node, pos0 + 32 * j);
-                            weigh(std::true_type{}, tmem + b * 128 + lanes, i, bits);
+                                hide(s_at + 32 * j, seq.n <= 128 ? tree_visible2(a, seq, node, pos0 + 32 * j, w0, w1) : tree_visible(a, seq, node, pos0 + 32 * j));
+                            tc_wait_st();
                         }
-                        clear_v(i, n, min(kTcKeys, len - pos0), max(0, ctx - pos0));
+                        weigh(s_at, i);
                     }
+                    if (masked) clear_v(i, n, min(kTcKeys, len - pos0), max(0, ctx - pos0));
                     begun = true;
                 }
                 if (pending) finish();  // its last product ran while this tile's weights were worked out
@@ -903,9 +911,9 @@ unsigned tree_tc_block(const TreeArgs& a) { return kTcRows / a.group * a.group; 
 
 size_t tree_tc_rows(const lokal_cuda_ctx* ctx) { return static_cast<size_t>(tc_shares(ctx)) * 2 * kTcRows; }
 
-// Rows the copy engine can take (16-byte grid), and a scale that does not turn a maximum into a minimum.
+// Rows the copy engine can take (16-byte grid), and a scale that leaves a maximum a maximum and -inf what it is.
 bool tree_tc_takes(const TreeArgs& a, int dtype, int kv_dtype) {
-    return dtype == kv_dtype && dtype != LOKAL_F32 && (a.head_dim == 64 || a.head_dim == 128) && a.group <= kTcRows && a.scale_log2 >= 0.0f && a.row_bytes % 16 == 0 && aligned_to(a.k, 16) &&
+    return dtype == kv_dtype && dtype != LOKAL_F32 && (a.head_dim == 64 || a.head_dim == 128) && a.group <= kTcRows && a.scale_log2 > 0.0f && a.row_bytes % 16 == 0 && aligned_to(a.k, 16) &&
            aligned_to(a.v, 16) && aligned_to(a.q, 16) && aligned_to(a.out, 16) && a.q_stride % 8 == 0 && a.out_stride % 8 == 0;
 }
 
