@@ -31,7 +31,6 @@ namespace {
 
 constexpr unsigned kMaxShares = 512;  // CTAs of the attention kernel, one per SM: more are not used
 constexpr int kTcRows = 128, kTcKeys = 128, kTcThreads = 384;
-constexpr unsigned kSoftmaxThreads = 256;
 
 template <int HD>
 struct TcShape {
@@ -306,7 +305,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (lane == 0) {
             for (unsigned i = 0; i < 2 * S::kSlots + S::kScores; i++) mbar_init(bars + i * 8, 1);
             for (unsigned b = 0; b < S::kScores; b++) {
-                mbar_init(pready(b), 128);
+                mbar_init(pready(b), 4);
                 mbar_init(sfree(b), 1);
             }
             for (unsigned b = 0; b < 2; b++) {
@@ -315,13 +314,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             mbar_init(udone, 1);
             for (unsigned i = 0; i < S::kUnits; i++) mbar_init(ufull + 8 * i, 1);
-            mbar_init(fbar, kSoftmaxThreads);
+            mbar_init(fbar, 8);
             mbar_init_fence();
             for (int i = 1; i < 6; i++) misc[i] = 0;
         }
     }
     if (warp == 9 && lane < 3) tma_prefetch(lane == 0 ? &map_q : lane == 1 ? &map_k : &map_v);
-    pdl_sync();
+    pdl_wait();
+    pdl_launch();  // only now: tree_join_tc_kernel looks at the lengths before it waits for this launch
     // the ring is not in use yet: its first bytes hold the sums of the walk
     const unsigned shares = gridDim.x;
     const TreePlace place = tree_locate<kTcKeys, kTcThreads>(a, reinterpret_cast<unsigned long long*>(tc_smem), blockIdx.x == 0, [&](unsigned total) {
@@ -543,7 +543,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // The two groups meet, twice for every block. (A wait that can give up, not a hardware barrier: were one group to
         // give up on something else, the other would stand there for good.)
         const auto meet = [&](unsigned phase) {
-            mbar_arrive(fbar);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(fbar);
             ok = __all_sync(0xffffffffu, tc_wait(fbar, phase, a.wait_limit, gave_up)) && ok;
         };
         // The two streams of a block are put together and written out.
@@ -675,19 +676,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         };
         // V rows behind the last position are cleared (they may hold anything, and 0 * NaN is NaN); so are drafted ones with an
         // infinity or a NaN, which rows that do not see them must not get: add_bad_values.
-        const auto clear_v = [&](unsigned i, unsigned n, int valid, int drafted) {
+        // `helpers` threads, this one number `me` of them, share it: the warps that have no rows, or all four.
+        const auto clear_v = [&](unsigned i, unsigned n, int valid, int drafted, unsigned me, unsigned helpers) {
             const unsigned at = 2 * t + v_place<HD>(i, n), slot = at % S::kSlots;
             ok = __all_sync(0xffffffffu, ok && tc_wait(full(slot), (at / S::kSlots) & 1u, a.wait_limit, gave_up));
             if (!ok) return;
             unsigned char* v_at = tc_smem + S::kRing + slot * S::kTile;
             const unsigned pieces = S::kSubs * 8;  // of 16 bytes, to a row
-            for (unsigned e = row; e < (kTcKeys - valid) * pieces; e += 128) {
+            for (unsigned e = me; e < (kTcKeys - valid) * pieces; e += helpers) {
                 const unsigned r = valid + e / pieces, c = e % pieces;
                 *reinterpret_cast<uint4*>(v_at + (c / 8) * S::kPanel + r * 128 + (c % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
             // eight threads to a panel row: a row is cleared by the threads that read it
-            const unsigned g8 = row >> 3, c8 = row & 7u;
-            for (int r0 = drafted; r0 < valid; r0 += 16) {
+            const unsigned g8 = me >> 3, c8 = me & 7u;
+            for (int r0 = drafted; r0 < valid; r0 += static_cast<int>(helpers >> 3)) {
                 const int r = r0 + static_cast<int>(g8);
                 bool bad = false;
                 if (r < valid) {
@@ -748,13 +750,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                         weigh(s_at, i);
                     }
-                    if (masked) clear_v(i, n, min(kTcKeys, len - pos0), max(0, ctx - pos0));
+                    if (masked) {
+                        const unsigned first = min((m_rows + 31) / 32, 4u) & 3u;  // warps 0 .. first - 1 have rows, unless all do
+                        if ((warp & 3u) >= first) clear_v(i, n, min(kTcKeys, len - pos0), max(0, ctx - pos0), row - first * 32, 128 - first * 32);
+                    }
                     begun = true;
                 }
                 if (pending) finish();  // its last product ran while this tile's weights were worked out
                 if (has) {
                     tc_fence_before();
-                    mbar_arrive(pready(b));
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(pready(b));
                 }
                 i += 2;
             } while (i < n);
@@ -774,20 +780,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 // Joins the pieces of blocks that several CTAs share. CTA c stands at the border between shares c and c + 1; the CTAs at
-// the borders inside one block (eight CTAs to a border) divide it among them in parts of 8 rows by 32 columns, a thread to
-// each value. The pieces' weights are worked out once for the rows at hand; eight pieces are in flight at a time.
+// the borders inside one block (eight CTAs to a border) divide it among them in parts of 8 rows by 32 columns, a thread to a
+// value, or, of more than eight pieces, 8 rows by 8 columns, four threads to a value with a quarter of the pieces each.
+// Eight pieces are in flight at a time. (Always by quarters, blocks of few pieces took 12 us longer over 128-row chunks;
+// never, one block in 148 pieces took 25 us longer.) The walk to the block is done while the
+// attention kernel still runs: what it reads was there before that kernel began.
 template <typename T>
 __global__ void __launch_bounds__(256) tree_join_tc_kernel(const TreeArgs a, unsigned shares) {
-    pdl_sync();
+    pdl_launch();
     __shared__ unsigned long long sh[2 * 8 + 4];
     __shared__ float weight[kMaxShares + 1][8];
     __shared__ float row_sum[8];
+    __shared__ float quarter[3][64];
     const unsigned c = blockIdx.x + 1;
     const TreePlace p = tree_locate<kTcKeys, 256>(a, sh, false, [&](unsigned total) {
         const TreeShares s(total, shares);
         return c < s.g ? s.first(c) : total;
     });
-    if (p.seq >= a.n_seqs) return;
+    if (p.seq >= a.n_seqs) {
+        pdl_wait();
+        return;
+    }
     const TreeShares s(p.total, shares);
     const unsigned border = s.first(c);
     const TreeSeq q = tree_seq(a, p.seq, false);
@@ -795,35 +808,37 @@ __global__ void __launch_bounds__(256) tree_join_tc_kernel(const TreeArgs a, uns
     const unsigned rows_all = q.n * a.group, blocks = (rows_all + a.block_rows - 1) / a.block_rows;
     const unsigned unit = (border - p.base) / kt;
     const unsigned t0 = p.base + unit * kt;
-    if (border == t0) return;
     const unsigned first = s.owner(t0) + 1, last = s.owner(t0 + kt - 1);  // borders inside the block
     const unsigned n_borders = last - first + 1, n_pieces = n_borders + 1;
     const unsigned kv_head = unit / blocks, block = unit - kv_head * blocks;
     const unsigned m_rows = min(a.block_rows, rows_all - block * a.block_rows);
-    const unsigned cols = a.head_dim / 32, parts = (m_rows + 7) / 8 * cols;
+    const unsigned slices = n_pieces > 8 ? 4u : 1u, part_cols = 32 / slices;
+    const unsigned cols = a.head_dim / part_cols, parts = (m_rows + 7) / 8 * cols;
     const unsigned mine = (c - first) * gridDim.y + blockIdx.y, of = n_borders * gridDim.y;
-    const unsigned part1 = parts * (mine + 1) / of;
+    const unsigned part0 = parts * mine / of, part1 = parts * (mine + 1) / of;
+    pdl_wait();
+    if (border == t0) return;
     // piece x (0 ..) is left by share first - 1 + x; only the first of them may be a CTA's second block
     const bool second = s.first(first - 1) < t0;
-    const auto piece = [&](unsigned x) { return static_cast<size_t>(first - 1 + x) * 2 + (x == 0 && second ? 1 : 0); };
-    const unsigned r = threadIdx.x & 7u, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const auto piece = [&](unsigned x) { return (first - 1 + x) * 2 + (x == 0 && second ? 1u : 0u); };
+    const unsigned r = threadIdx.x & 7u, in_part = (threadIdx.x >> 3) % part_cols, slice = threadIdx.x / (8 * part_cols), lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     unsigned rows_at = 0xffffffffu;
-    for (unsigned part = parts * mine / of; part < part1; part++) {
-        const unsigned row0 = part / cols * 8, col = part % cols * 32 + (threadIdx.x >> 3);
+    for (unsigned part = part0; part < part1; part++) {
+        const unsigned row0 = part / cols * 8, col = part % cols * part_cols + in_part;
+        if (slices > 1 || row0 != rows_at) __syncthreads();  // what the part before left in shared memory has been read
         if (row0 != rows_at) {
             // a warp takes a row: the largest maximum, then the weights and their sum
             rows_at = row0;
-            __syncthreads();
             const bool in = row0 + warp < m_rows;
             float top = -INFINITY, l = 0.0f;
             if (in)
-                for (unsigned x = lane; x < n_pieces; x += 32) top = fmaxf(top, a.part_ml[piece(x) * kTcRows + row0 + warp].x);
+                for (unsigned x = lane; x < n_pieces; x += 32) top = fmaxf(top, a.part_ml[static_cast<size_t>(piece(x)) * kTcRows + row0 + warp].x);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             for (unsigned x = lane; x < n_pieces; x += 32) {
                 float w = 0.0f;  // stays 0 where nothing of a piece was visible
                 if (in) {
-                    const float2 ml = a.part_ml[piece(x) * kTcRows + row0 + warp];
+                    const float2 ml = a.part_ml[static_cast<size_t>(piece(x)) * kTcRows + row0 + warp];
                     if (ml.y != 0.0f) {
                         w = ex2(ml.x - (top == -INFINITY ? 0.0f : top));
                         l = fmaf(ml.y, w, l);
@@ -836,14 +851,21 @@ __global__ void __launch_bounds__(256) tree_join_tc_kernel(const TreeArgs a, uns
             __syncthreads();
         }
         const unsigned row = row0 + r;
-        if (row >= m_rows) continue;
         float acc = 0.0f;
+        if (row < m_rows) {
+            const unsigned x1 = n_pieces * (slice + 1) / slices;
 #pragma unroll 8
-        for (unsigned x = 0; x < n_pieces; x++) {
-            const float w = weight[x][r];
-            const float o = a.part_o[piece_at(piece(x), a.head_dim, col, row)];
-            acc = w == 0.0f ? acc : fmaf(o, w, acc);
+            for (unsigned x = n_pieces * slice / slices; x < x1; x++) {
+                const float w = weight[x][r], o = a.part_o[piece_at(piece(x), a.head_dim, col, row)];
+                acc = w == 0.0f ? acc : fmaf(o, w, acc);
+            }
         }
+        if (slices > 1) {
+            if (slice) quarter[slice - 1][threadIdx.x & 63u] = acc;
+            __syncthreads();
+            if (slice == 0) acc = ((acc + quarter[0][threadIdx.x]) + quarter[1][threadIdx.x]) + quarter[2][threadIdx.x];
+        }
+        if (slice || row >= m_rows) continue;
         const unsigned flat = block * a.block_rows + row, node = flat / a.group, head = kv_head * a.group + flat % a.group;
         const float l = row_sum[r];
         static_cast<T*>(a.out)[static_cast<size_t>(q.row0 + node) * a.out_stride + static_cast<size_t>(head) * a.head_dim + col] = from_f32<T>(l == 0.0f ? 0.0f : acc / l);
