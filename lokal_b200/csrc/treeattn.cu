@@ -351,8 +351,13 @@ int lokal_cuda_tree_plan(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const lokal_k
 
 size_t lokal_cuda_tree_attn_workspace(const lokal_cuda_ctx* ctx, size_t rows, uint32_t n_q_heads, uint32_t n_kv_heads, uint32_t head_dim) {
     if (!ctx || rows == 0 || n_q_heads == 0 || n_kv_heads == 0 || head_dim == 0 || head_dim > 256) return 0;
-    const size_t any = lokal::any_rows(ctx, head_dim), tc = head_dim == 64 || head_dim == 128 ? lokal::tree_tc_rows(ctx) : 0;
-    return (any > tc ? any : tc) * (head_dim + 2) * sizeof(float);
+    size_t most = lokal::any_rows(ctx, head_dim);
+    if (head_dim == 64 || head_dim == 128) {
+        const size_t tc = lokal::tree_tc_rows(ctx), mma = lokal::tree_mma_rows(ctx, head_dim);
+        if (tc > most) most = tc;
+        if (mma > most) most = mma;
+    }
+    return most * (head_dim + 2) * sizeof(float);
 }
 
 int lokal_cuda_tree_attn(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const lokal_kv_pool* pool, uint32_t k_store, uint32_t v_store,
@@ -404,12 +409,13 @@ int lokal_cuda_tree_attn(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const lokal_k
     a.scale_log2 = scale * 1.4426950408889634f;
     a.wait_limit = static_cast<unsigned>(lokal::tune_env("LOKAL_CUDA_WAIT_LIMIT", lokal::kWaitLimit));
     cudaStream_t st = static_cast<cudaStream_t>(s);
-    const bool tc = lokal::tree_tc_takes(a, dtype, kv_dtype);
     a.out_vec32 = lokal::aligned_to(out, 32) && out_row_stride * es % 32 == 0;
-    a.block_rows = tc ? lokal::tree_tc_block(a) : lokal::kAnyRows;
+    const bool tc = lokal::tree_tc_takes(a, dtype, kv_dtype), mma = !tc && lokal::tree_mma_takes(a, dtype, kv_dtype);
+    a.block_rows = tc ? lokal::tree_tc_block(a) : 16u;
     a.part_ml = static_cast<float2*>(workspace);
-    a.part_o = reinterpret_cast<float*>(a.part_ml + (tc ? lokal::tree_tc_rows(ctx) : lokal::any_rows(ctx, head_dim)));
+    a.part_o = reinterpret_cast<float*>(a.part_ml + (tc ? lokal::tree_tc_rows(ctx) : mma ? lokal::tree_mma_rows(ctx, head_dim) : lokal::any_rows(ctx, head_dim)));
     if (tc) return lokal::launch_tree_tc(ctx, st, a, dtype);
+    if (mma) return lokal::launch_tree_mma(ctx, st, a, dtype, kv_dtype);
     switch (dtype) {
         case LOKAL_F32: return lokal::launch_any_q<float>(ctx, st, a, kv_dtype);
         case LOKAL_F16: return lokal::launch_any_q<__half>(ctx, st, a, kv_dtype);

@@ -1,4 +1,4 @@
-// What the two attention kernels (treeattn.cu: any type and shape; treeattn_tc.cu: 16-bit rows on the tensor cores) and
+// What the three attention kernels (treeattn_tc.cu: 16-bit rows; treeattn_mma.cu: f32 accuracy; treeattn.cu: the rest) and
 // the launch that joins their pieces share: the arguments, the walk over the work, the visibility of drafted rows.
 //
 // The work of a call is a list of tiles: for every sequence, key head and block of up to R query rows (a row is one drafted
@@ -294,6 +294,10 @@ bool tree_tc_takes(const TreeArgs& a, int dtype, int kv_dtype);
 unsigned tree_tc_block(const TreeArgs& a);
 size_t tree_tc_rows(const lokal_cuda_ctx* ctx);
 int launch_tree_tc(lokal_cuda_ctx* ctx, cudaStream_t s, const TreeArgs& a, int dtype);
+// The kernel with f32 accuracy on the tensor cores (treeattn_mma.cu).
+bool tree_mma_takes(const TreeArgs& a, int dtype, int kv_dtype);
+size_t tree_mma_rows(const lokal_cuda_ctx* ctx, unsigned head_dim);
+int launch_tree_mma(lokal_cuda_ctx* ctx, cudaStream_t s, const TreeArgs& a, int dtype, int kv_dtype);
 
 // Joins the pieces of blocks that several CTAs share. CTA c stands at the border between shares c and c + 1; the CTAs at
 // the borders inside one block divide its rows among them. A warp takes a row, or, where a CTA has fewer rows than warps,
