@@ -38,6 +38,7 @@ struct PoolWork {
     int* ent_new;    // [n_slots] per entry: its first place in free_list, -1 = skipped
     int* ent_len;    // [n_slots] per entry: positions of the slot before the call (fork: of the source)
     int* ent_cow;    // [n_slots] per entry: page that is copied before the slot writes to it, -1 = none
+    int* arrived;    // [n_slots] accept: CTAs of a sequence that are done; 0 between calls
 };
 
 __host__ __device__ inline PoolWork pool_work(int* w, unsigned n_pages, unsigned n_slots) {
@@ -54,9 +55,10 @@ __host__ __device__ inline PoolWork pool_work(int* w, unsigned n_pages, unsigned
     p.ent_new = p.claim + n_slots;
     p.ent_len = p.ent_new + n_slots;
     p.ent_cow = p.ent_len + n_slots;
+    p.arrived = p.ent_cow + n_slots;
     return p;
 }
-inline size_t pool_work_ints(unsigned n_pages, unsigned n_slots) { return 4 + 5 * static_cast<size_t>(n_pages) + 4 * static_cast<size_t>(n_slots); }
+inline size_t pool_work_ints(unsigned n_pages, unsigned n_slots) { return 4 + 5 * static_cast<size_t>(n_pages) + 5 * static_cast<size_t>(n_slots); }
 
 // Exclusive prefix sum over the CTA (kPlanThreads threads) of one value per thread; `total` for everybody.
 template <typename N>
@@ -301,24 +303,26 @@ __global__ void __launch_bounds__(256) pool_apply_kernel(const PoolArgs a, const
     run_copies<V>(a, w.copy_src, w.copy_dst, w.copy_rows, static_cast<unsigned>(*w.n_copies));
 }
 
-// Pages behind the first ceil(new_len / page_rows) are given back. A table entry is taken out by an exchange, so that a
-// slot which the list names twice gives every page back once.
+// Page p of a slot is given back if no position below `want` lies in it. The table entry is taken out by an exchange, so
+// that a slot which a list names twice gives every page back once.
+__device__ __forceinline__ void give_back(const PoolArgs& a, unsigned slot, unsigned p, int want) {
+    if (static_cast<long long>(p) << a.page_shift < want) return;
+    const int old = atomicExch(a.table + static_cast<size_t>(slot) * a.max_pages + p, -1);
+    if (page_ok(a, old)) atomicSub(a.refs + old, 1);
+}
+
 __global__ void __launch_bounds__(256) pool_truncate_kernel(const PoolArgs a, const ListArgs l) {
     pdl_sync();
     const unsigned i = blockIdx.y;
     const unsigned slot = l.dst[i];
     const int want = l.new_lens ? l.new_lens[i] : 0;
     if (slot >= a.n_slots || want < 0) {
-        if (threadIdx.x == 0 && blockIdx.x == 0 && slot >= a.n_slots) atomicOr(a.err_word, kErrPageRange);
-        if (threadIdx.x == 0 && blockIdx.x == 0 && want < 0 && !l.src) atomicOr(a.err_word, kErrPageRange);
+        if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(a.err_word, kErrPageRange);
         return;
     }
     const unsigned p = blockIdx.x * 256 + threadIdx.x;
     if (p == 0) atomicMin(a.lens + slot, want);
-    if (p >= a.max_pages) return;
-    if (static_cast<long long>(p) << a.page_shift < want) return;
-    const int old = atomicExch(a.table + static_cast<size_t>(slot) * a.max_pages + p, -1);
-    if (page_ok(a, old)) atomicSub(a.refs + old, 1);
+    if (p < a.max_pages) give_back(a, slot, p, want);
 }
 
 // The k-th free page below n_used gets the k-th used page at or above n_used: as many of one as of the other, sources
@@ -448,12 +452,10 @@ __global__ void __launch_bounds__(256) pool_accept_kernel(const PoolArgs a, cons
     }
     __syncthreads();
     ok = ok && !bad;
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        w.ent_len[i] = ok ? base + count : -1;  // the length the cut that follows leaves, -1 = leave the slot alone
-        w.ent_new[i] = static_cast<int>(slot);
-        if (!ok) atomicOr(a.err_word, kErrPageRange);
+    if (!ok) {
+        if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.err_word, kErrPageRange);
+        return;
     }
-    if (!ok) return;
     const unsigned row_vecs = static_cast<unsigned>(a.row_bytes / sizeof(V));
     const unsigned long long vecs = static_cast<unsigned long long>(row_vecs) * a.n_stores;
     for (unsigned long long e = static_cast<unsigned long long>(blockIdx.x) * 256 + threadIdx.x; e < vecs; e += gridDim.x * 256ull) {
@@ -469,6 +471,20 @@ __global__ void __launch_bounds__(256) pool_accept_kernel(const PoolArgs a, cons
                 if (j0 + j < count && from[j0 + j] != to[j0 + j]) base_v[static_cast<size_t>(to[j0 + j]) * row_vecs] = v[j];
         }
     }
+    // The cut behind the path: by the sequence's last CTA, when all have read the table (and in the one launch that the
+    // moves need; the count is back at 0 for the next call).
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        bad = atomicAdd(w.arrived + i, 1) == static_cast<int>(gridDim.x) - 1;
+    }
+    __syncthreads();
+    if (!bad) return;
+    if (threadIdx.x == 0) {
+        w.arrived[i] = 0;
+        a.lens[slot] = base + count;
+    }
+    for (unsigned p = threadIdx.x; p < a.max_pages; p += 256) give_back(a, slot, p, base + count);
 }
 
 // ---- cache rows of token rows, the paged twin of kv_rows ----
@@ -587,6 +603,7 @@ int lokal_cuda_kv_pool_create(lokal_cuda_ctx* ctx, uint32_t page_rows, uint32_t 
     void* dev = nullptr;
     cudaError_t e = p->stores ? cudaSuccess : cudaErrorMemoryAllocation;
     if (e == cudaSuccess) e = cudaMalloc(&dev, n_stores * sizeof(void*) + ints * sizeof(int));
+    if (e == cudaSuccess) e = cudaMemset(dev, 0, n_stores * sizeof(void*) + ints * sizeof(int));
     if (e == cudaSuccess) e = cudaMemcpy(dev, stores, n_stores * sizeof(void*), cudaMemcpyHostToDevice);
     if (e != cudaSuccess) {
         if (dev) cudaFree(dev);
@@ -714,10 +731,7 @@ int lokal_cuda_kv_pool_accept(lokal_cuda_ctx* ctx, lokal_cuda_stream s, lokal_kv
     if (pool->vec16) lokal::launch_k(lokal::pool_accept_kernel<uint4>, grid, 256, 0, st, lokal::args_of(ctx, pool), t);
     else lokal::launch_k(lokal::pool_accept_kernel<unsigned short>, grid, 256, 0, st, lokal::args_of(ctx, pool), t);
     LOKAL_CHECK_LAUNCH(ctx, "pool_accept_kernel");
-    const lokal::PoolWork w = lokal::pool_work(pool->a.work, pool->a.n_pages, pool->a.n_slots);
-    // `src` marks the list as the one the launch above has written: -1 there is a sequence it has reported already
-    const lokal::ListArgs l{reinterpret_cast<const uint32_t*>(w.ent_new), reinterpret_cast<const uint32_t*>(w.ent_new), w.ent_len, t.n_seqs};
-    return lokal::launch_truncate(ctx, st, pool, l);
+    return LOKAL_OK;
 }
 
 }  // extern "C"

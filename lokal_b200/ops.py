@@ -18,12 +18,14 @@ from .capi import BF16, F16, F32, Q4_K, Q8_0, KvLayout, LokalCudaError, PassConf
 
 
 def _ptr(x):
-    if x is None:
-        return None
+    if x is None or type(x) is int:
+        return x
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        pass
     if isinstance(x, int):
         return x
-    if hasattr(x, "data_ptr"):
-        return x.data_ptr()
     if isinstance(x, np.ndarray):
         return x.ctypes.data
     raise TypeError(f"cannot take the address of {type(x)!r}")
