@@ -408,6 +408,7 @@ int lokal_cuda_tree_attn(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const lokal_k
     a.head_dim = head_dim;
     a.scale_log2 = scale * 1.4426950408889634f;
     a.wait_limit = static_cast<unsigned>(lokal::tune_env("LOKAL_CUDA_WAIT_LIMIT", lokal::kWaitLimit));
+    a.extra_tx = static_cast<unsigned>(lokal::tune_env("LOKAL_CUDA_TEST_EXTRA_TX", 0));
     cudaStream_t st = static_cast<cudaStream_t>(s);
     a.out_vec32 = lokal::aligned_to(out, 32) && out_row_stride * es % 32 == 0;
     const bool tc = lokal::tree_tc_takes(a, dtype, kv_dtype), mma = !tc && lokal::tree_mma_takes(a, dtype, kv_dtype);

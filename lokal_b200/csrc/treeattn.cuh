@@ -30,7 +30,7 @@ struct TreeArgs {
     unsigned n_seqs, rows, mask_words, n_q_heads, n_kv_heads, group, head_dim;
     unsigned page_rows, page_shift, n_pages, n_slots, max_pages;
     unsigned block_rows;  // query rows of a block: at most R
-    unsigned wait_limit;
+    unsigned wait_limit, extra_tx;  // polls before a wait gives up; bytes announced that do not come (for the test of that)
     int out_vec32;        // rows of out start on 32-byte boundaries
     float scale_log2;  // scale * log2(e): the exponentials are powers of two
 };

@@ -211,6 +211,8 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 
 __device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
+constexpr unsigned kDrainPolls = 1u << 14;  // for what is in flight when a wait has given up: it lands in microseconds
+
 // A wait that gives up: after `limit` polls, or when another role of the CTA has.
 __device__ __forceinline__ bool tc_wait(uint32_t mbar, unsigned parity, unsigned limit, volatile int* gave_up) {
     if (mbar_try_wait(mbar, parity)) return true;
@@ -412,7 +414,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 const unsigned mine = __shfl_sync(0xffffffffu, pages, min(page - page0 + lane, 31u));
                 const int y = static_cast<int>((mine << a.page_shift) + (pos & (a.page_rows - 1)));
-                if (lane == 0) mbar_expect_tx(full(at.slot), boxes * box_rows * 128 * S::kSubs);
+                if (lane == 0) mbar_expect_tx(full(at.slot), boxes * box_rows * 128 * S::kSubs + a.extra_tx);
                 __syncwarp();
                 if (lane < boxes) {
                     const uint32_t to = smem + S::kRing + at.slot * S::kTile + lane * box_rows * 128;
@@ -427,11 +429,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
         }
         if (!ok && place.seq < a.n_seqs) {
-            // what is in flight lands before the CTA gives its memory back
+            // what is in flight lands before the CTA gives its memory back (however soon the wait before gave up)
             for (unsigned slot = 0; slot < S::kSlots; slot++)
-                if ((issued >> slot) & 1u) mbar_wait_bounded(full(slot), (parity >> slot) & 1u, a.wait_limit);
+                if ((issued >> slot) & 1u) mbar_wait_bounded(full(slot), (parity >> slot) & 1u, kDrainPolls);
             if (!is_k) {
-                for (unsigned q = q_blocks > 2 ? q_blocks - 2 : 0u; q < q_blocks; q++) mbar_wait_bounded(qfull + 8 * (q & 1u), (q >> 1) & 1u, a.wait_limit);
+                for (unsigned q = q_blocks > 2 ? q_blocks - 2 : 0u; q < q_blocks; q++) mbar_wait_bounded(qfull + 8 * (q & 1u), (q >> 1) & 1u, kDrainPolls);
             }
         }
     } else if (warp == 9) {
@@ -482,7 +484,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (ok) publish(0);
         if (!ok && place.seq < a.n_seqs) {
             // the products in flight end before TMEM is given back
-            if (t) mbar_wait_bounded(sfull((t - 1) % S::kScores), ((t - 1) / S::kScores) & 1u, a.wait_limit);
+            if (t) mbar_wait_bounded(sfull((t - 1) % S::kScores), ((t - 1) / S::kScores) & 1u, kDrainPolls);
         }
     } else if (warp == 10) {
         // ---- O += P V ----
@@ -527,7 +529,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!ok && place.seq < a.n_seqs) {
             // the products in flight end before TMEM is given back
             if (tc_elect()) tc_commit(udone);
-            mbar_wait_bounded(udone, units & 1u, a.wait_limit);
+            mbar_wait_bounded(udone, units & 1u, kDrainPolls);
         }
     } else {
         // ---- softmax ----

@@ -523,3 +523,94 @@ def test_draft_verify_accept_steps(ctx, dev, dtype, kv):
         ctx.stream_sync()
         assert list(lens.cpu().numpy()[:3]) == [len(held[s]) for s in slots]
     pool.close()
+
+
+# ---- what only large or unusual calls reach ----
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,hd", [(BF16, 128), (F16, 64), (F32, 128)])
+def test_rows_past_four_gigabytes(ctx, dev, dtype, hd):
+    """Pages at the far end of a store of 5 GB (one store is K and V at once): byte offsets need more than 32 bits."""
+    import torch
+    hkv, page = 8, 64
+    c = Case(ctx, dev, lens=[300, 70], drafts=[9, 70], hq=8, hkv=hkv, hd=hd, page=page, dtype=dtype, kv=dtype, seed=101)
+    row_bytes = hkv * hd * (4 if dtype == F32 else 2)
+    far = 5 * 2 ** 30 // (page * row_bytes)
+    d = c.upload()
+    big = torch.empty(((far + c.n_pages) * page, hkv * hd), dtype=d["k"].dtype, device="cuda")
+    big[far * page:] = d["k"]
+    c.v = c.k
+    pool = L.KvPool(ctx, page_rows=page, n_pages=far + c.n_pages, n_slots=c.n_slots, max_pages=c.max_pages, table=d["table"] + far * (d["table"] >= 0).int(),
+                    lens=d["lens"], refs=torch.zeros(far + c.n_pages, dtype=torch.int32, device="cuda"), stores=[big], row_bytes=row_bytes)
+    ctx.tree_attn(pool, d["q"], d["out"], k_store=0, v_store=0, slots=d["slots"], q_start=d["starts"], n_seqs=2, rows=c.rows, mask=d["mask"],
+                  mask_words=c.words, n_q_heads=8, n_kv_heads=hkv, head_dim=hd, scale=c.scale, dtype=dtype, kv_dtype=dtype, workspace=d["work"],
+                  workspace_bytes=d["bytes"])
+    ctx.stream_sync()
+    c.check(dev.get(d["out"]))
+    # and pages are copied there and back
+    pair = lambda *x: dev.put(np.array(x, np.int32))
+    pool.copy_pages(pair(far, far + 1), pair(0, far + c.n_pages - 1), n=2)
+    ctx.stream_sync()
+    assert torch.equal(big[:page], big[far * page:(far + 1) * page])
+    assert torch.equal(big[-page:], big[(far + 1) * page:(far + 2) * page])
+    pool.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv,hd", [(BF16, BF16, 64), (F16, F16, 128), (F32, F16, 128), (F32, F32, 64)])
+def test_more_sequences_than_a_walk_remembers(ctx, dev, dtype, kv, hd):
+    # thousands of short sequences: each CTA steps through more of them than fit its shared memory, and a block is one tile
+    rng = np.random.default_rng(7)
+    n = 6000
+    drafts = rng.integers(0, 3, n)
+    drafts[0] = 2
+    c = Case(ctx, dev, lens=drafts + rng.integers(1, 20, n), drafts=drafts, hq=2, hkv=1, hd=hd, page=8, dtype=dtype, kv=kv, seed=103)
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv,hd", [(BF16, BF16, 64), (BF16, BF16, 128), (F32, F16, 64)])
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+def test_scales_that_are_negative_or_zero(ctx, dev, dtype, kv, hd, scale):
+    c = Case(ctx, dev, lens=[200, 33], drafts=[7, 33], hq=4, hkv=2, hd=hd, dtype=dtype, kv=kv, scale=scale, seed=105)
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drafts", [120, 128, 129, 300])
+def test_sequences_with_more_drafted_rows_than_a_tile(ctx, dev, drafts):
+    # masks of two words and of more, trees that reach over several key tiles and blocks of rows
+    for dtype in (BF16, F32):
+        c = Case(ctx, dev, lens=[drafts + 61, drafts], drafts=[drafts, drafts], hq=6, hkv=2, hd=64, dtype=dtype, kv=dtype, mask="tree", seed=drafts)
+        c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_a_wait_that_runs_out_is_an_error_and_the_next_call_is_right(ctx, dev, monkeypatch, hd):
+    # the copies announce 16 bytes more than they bring (as in tests/test_gpu_timeout.py): every wait for one gives up
+    c = Case(ctx, dev, lens=[3000, 500], drafts=[9, 5], hq=4, hkv=2, hd=hd, dtype=BF16, kv=BF16, seed=107)
+    c.upload()
+    monkeypatch.setenv("LOKAL_CUDA_TEST_EXTRA_TX", "16")
+    monkeypatch.setenv("LOKAL_CUDA_WAIT_LIMIT", "200")
+    c.call()
+    with pytest.raises(L.LokalCudaError) as e:
+        ctx.stream_sync()
+    assert e.value.status == capi.ERR_TIMEOUT
+    monkeypatch.delenv("LOKAL_CUDA_WAIT_LIMIT")
+    monkeypatch.delenv("LOKAL_CUDA_TEST_EXTRA_TX")
+    c.d["out"].fill_(c.fill)
+    c.call()
+    ctx.stream_sync()
+    c.check(dev.get(c.d["out"]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv,hd", [(BF16, BF16, 128), (F16, F16, 64), (F32, F16, 64), (F32, F32, 40)])
+def test_the_same_bits_every_time(ctx, dev, dtype, kv, hd):
+    c = Case(ctx, dev, lens=[5000, 900, 77], drafts=[20, 3, 40], hq=4, hkv=2, hd=hd, dtype=dtype, kv=kv, seed=109)
+    first = c.run()
+    for _ in range(5):
+        c.call()
+        ctx.stream_sync()
+        assert np.array_equal(dev.get(c.d["out"]), first)
