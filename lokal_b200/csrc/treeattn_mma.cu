@@ -24,8 +24,14 @@ struct Split {  // whether a value of the type needs a second tf32 part
     static constexpr bool value = sizeof(T) == 4;
 };
 
-__device__ __forceinline__ uint32_t tf32_hi(float x) { return __float_as_uint(x) & 0xffffe000u; }
-__device__ __forceinline__ uint32_t tf32_lo(float x, uint32_t hi) { return __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u; }
+// Both parts are rounded, not cut off: half a step of 2^-12 each instead of a whole one that always points to zero.
+__device__ __forceinline__ uint32_t tf32_round(float x) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t tf32_hi(float x) { return tf32_round(x); }
+__device__ __forceinline__ uint32_t tf32_lo(float x, uint32_t hi) { return tf32_round(x - __uint_as_float(hi)); }
 
 // c += a b over a contraction of 8: a 16 x 8, b 8 x 8
 __device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -160,9 +166,12 @@ __global__ void __launch_bounds__(kMmaThreads, HD == 64 ? 4 : 2) tree_attn_mma_k
                     for (int r = 0; r < VR; r++) vr[n][h][r] = load_run<(HD / 8 < E)>(at + r * 32);
                 }
             }
-            float z[NT][4];
+            // In several sums, put together in f32: a tensor core cuts a sum off where f32 would round it, and one long chain
+            // of products shows it (f32 over f32 with 128 columns: 1.2e-6 of the result, 0.33e-6 so).
+            constexpr int CH = NT == 1 ? 4 : 2;
+            float zs[CH][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; n++) z[n][0] = z[n][1] = z[n][2] = z[n][3] = 0.0f;
+            for (int n = 0; n < NT * CH; n++) zs[n / NT][n % NT][0] = zs[n / NT][n % NT][1] = zs[n / NT][n % NT][2] = zs[n / NT][n % NT][3] = 0.0f;
 #pragma unroll
             for (int s = 0; s < SUP; s++) {
 #pragma unroll
@@ -174,11 +183,18 @@ __global__ void __launch_bounds__(kMmaThreads, HD == 64 ? 4 : 2) tree_attn_mma_k
                     for (int n = 0; n < NT; n++) {
                         const float k0 = elem<TK>(kr[n][s], 2 * t), k1 = elem<TK>(kr[n][s], 2 * t + 1);
                         const uint32_t h0 = SK ? tf32_hi(k0) : __float_as_uint(k0), h1 = SK ? tf32_hi(k1) : __float_as_uint(k1);
-                        if (SQ) mma_tf32(z[n], lo.x, lo.y, lo.z, lo.w, h0, h1);
-                        if (SK) mma_tf32(z[n], hi.x, hi.y, hi.z, hi.w, tf32_lo(k0, h0), tf32_lo(k1, h1));
-                        mma_tf32(z[n], hi.x, hi.y, hi.z, hi.w, h0, h1);
+                        float(&zc)[4] = zs[(s * (E / 2) + t) % CH][n];
+                        if (SQ) mma_tf32(zc, lo.x, lo.y, lo.z, lo.w, h0, h1);
+                        if (SK) mma_tf32(zc, hi.x, hi.y, hi.z, hi.w, tf32_lo(k0, h0), tf32_lo(k1, h1));
+                        mma_tf32(zc, hi.x, hi.y, hi.z, hi.w, h0, h1);
                     }
                 }
+            }
+            float z[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) z[n][i] = CH == 4 ? (zs[0][n][i] + zs[1][n][i]) + (zs[2 % CH][n][i] + zs[3 % CH][n][i]) : zs[0][n][i] + zs[1][n][i];
             }
             const unsigned next = pos + 4 * kStep;
             if (next < pos_end) {
