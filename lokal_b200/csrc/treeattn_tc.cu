@@ -16,6 +16,13 @@
 // of products have a warp each because issuing them is what costs: one warp for both took 2150 clocks a tile of head size
 // 64, half as much again as the copy of the tile. So have the copies: a tile's boxes took one warp 600 clocks for K, 600 for V.
 // K and V tiles have their places in one ring in the order of their use.
+// A block of up to 16 rows (single tokens, small trees) wastes a tile of 128: every score costs its exponential, and the
+// warps whose lanes hold the rows compute 128 keys by 32 rows in turn. With head size 64, and where sequences have few rows on
+// average, such blocks are taken by the softmax warps themselves: products of 16 rows by 32 keys a warp, from the same ring,
+// every key's weight in a thread of its own (few_rows). Single tokens of 256 sequences of up to 4,096 keys, 32 heads over 4:
+// 181 us before, 148 so; 8 of 131,072 keys: 212 and 183 (5.9 TB/s). What it costs: blocks end slower (one key tile to a
+// sequence: 46 us before, 54), larger blocks in the same call run 6 % slower, and with head size 128, where a tile's copy takes
+// twice the time, it won 3 % at best and lost 25 % at short lengths, so those keep to the other way.
 // An accumulator is rescaled only when the maximum has grown by more than 2^8 since it was last set: weights then stay
 // below 2^8, which neither 16-bit type nor the f32 sums mind.
 // Weights are rounded to the cache's type for the product (half a step each, as the values they multiply were); sums,
@@ -31,6 +38,7 @@ namespace {
 
 constexpr unsigned kMaxShares = 512;  // CTAs of the attention kernel, one per SM: more are not used
 constexpr int kTcRows = 128, kTcKeys = 128, kTcThreads = 384;
+constexpr unsigned kFewRows = 16;  // blocks of up to so many rows take the products of a warp
 
 template <int HD>
 struct TcShape {
@@ -53,10 +61,30 @@ struct TcShape {
     static_assert(kScores * 128 + 2 * HD <= 512, "TMEM columns");
 };
 
+// Where the barriers are.
+template <int HD>
+struct TcBars {
+    using S = TcShape<HD>;
+    uint32_t at;
+    __device__ __forceinline__ uint32_t full(unsigned slot) const { return at + slot * 8; }
+    __device__ __forceinline__ uint32_t empty(unsigned slot) const { return at + (S::kSlots + slot) * 8; }
+    __device__ __forceinline__ uint32_t sfull(unsigned b) const { return at + (2 * S::kSlots + b) * 8; }                    // scores are there
+    __device__ __forceinline__ uint32_t pready(unsigned b) const { return at + (2 * S::kSlots + S::kScores + b) * 8; }      // weights are there
+    __device__ __forceinline__ uint32_t sfree(unsigned b) const { return at + (2 * S::kSlots + 2 * S::kScores + b) * 8; }   // weights have been used
+    __device__ __forceinline__ uint32_t qfull() const { return at + (2 * S::kSlots + 3 * S::kScores) * 8; }                 // Q tiles 0 and 1 each; qfree behind
+    __device__ __forceinline__ uint32_t udone() const { return qfull() + 32; }                                              // the last product of a block
+    __device__ __forceinline__ uint32_t ufull() const { return udone() + 8; }                                               // a block is described
+    __device__ __forceinline__ uint32_t fbar() const { return ufull() + 8 * S::kUnits; }                                    // the softmax groups meet
+};
+
 // A slot of the ring and the parity of its round.
 template <int HD>
 struct RingAt {
     unsigned slot = 0, round = 0;
+    __device__ __forceinline__ void skip(unsigned k) {  // any number
+        round ^= k / TcShape<HD>::kSlots & 1u;
+        add(k % TcShape<HD>::kSlots);
+    }
     __device__ __forceinline__ void add(unsigned k) {  // at most a round
         slot += k;
         if (slot >= TcShape<HD>::kSlots) {
@@ -72,6 +100,13 @@ template <int HD>
 __device__ __forceinline__ unsigned v_place(unsigned i, unsigned n) {
     return min(i + TcShape<HD>::kAhead + 1u, n) + i;
 }
+template <int HD>
+__device__ __forceinline__ unsigned k_place(unsigned i) {
+    return i + (i > TcShape<HD>::kAhead ? i - TcShape<HD>::kAhead : 0u);
+}
+
+// Rows of a block.
+__device__ __forceinline__ unsigned rows_of(const TreeArgs& a, unsigned drafted, unsigned block) { return min(a.block_rows, drafted * a.group - block * a.block_rows); }
 
 // ---- tcgen05 ----
 __device__ __forceinline__ void tc_alloc(uint32_t dst, unsigned cols) {
@@ -167,6 +202,31 @@ __device__ __forceinline__ constexpr uint32_t tc_idesc(unsigned fmt, unsigned n,
     return (1u << 4) | (fmt << 7) | (fmt << 10) | (b_mn << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
+// ---- products of a warp (blocks of few rows) ----
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : TC_R4(r, 0) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : TC_R4(r, 0) : "r"(at) : "memory");
+}
+// c += a b over a contraction of 16: a 16 x 16, b 16 x 8
+template <typename T>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (std::is_same<T, __half>::value)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : TC_W4(a, 0), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : TC_W4(a, 0), "r"(b0), "r"(b1));
+}
+// A 16-byte piece of a tile in shared memory: panels of 64 columns, rows of 128 bytes, the 128-byte swizzle.
+__device__ __forceinline__ uint32_t piece_of(uint32_t tile, unsigned row, unsigned chunk) {
+    return tile + (chunk >> 3) * (128u * 128u) + row * 128u + (((chunk ^ row) & 7u) << 4);
+}
+
+__device__ __forceinline__ void mbar_arrive_n(uint32_t mbar, unsigned n) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(mbar), "r"(n) : "memory"); }
 __device__ __forceinline__ void mbar_arrive(uint32_t mbar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(mbar) : "memory"); }
 __device__ __forceinline__ bool mbar_is_done(uint32_t mbar, unsigned parity) {  // a look, without waiting
     unsigned yes;
@@ -196,11 +256,19 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// whether one of the two values is an infinity or a NaN
+// the two values, 0 for one that is an infinity or a NaN
 template <typename T>
-__device__ __forceinline__ bool bad_pair(uint32_t v) {
+__device__ __forceinline__ uint32_t finite_pair(uint32_t v) {
     constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-    return (v & e) == e || ((v >> 16) & e) == e;
+    return ((v & e) == e ? 0u : v & 0xffffu) | (((v >> 16) & e) == e ? 0u : v & 0xffff0000u);
+}
+// Eight values in shared memory without their infinities and NaNs; whether there were any.
+template <typename T>
+__device__ __forceinline__ bool make_finite(uint4* p) {
+    const uint4 x = *p, y = make_uint4(finite_pair<T>(x.x), finite_pair<T>(x.y), finite_pair<T>(x.z), finite_pair<T>(x.w));
+    if (x.x == y.x && x.y == y.y && x.z == y.z && x.w == y.w) return false;
+    *p = y;
+    return true;
 }
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t mbar) {
@@ -249,7 +317,7 @@ struct __align__(16) TcUnit {
     __device__ int ctx() const { return static_cast<int>(len - drafted); }
 };
 
-// V rows that hold an infinity or a NaN and belong to drafted rows were cleared for the product, because rows that do not
+// Infinities and NaNs in V rows of drafted rows were set to 0 for the product, because rows that do not
 // see them would get 0 * inf. What they add to the rows that do see them is added here, to the stored result: rare, and
 // slow (a dot product per row and value).
 template <typename T, int HD>
@@ -282,7 +350,255 @@ __device__ __noinline__ void add_bad_values(const TreeArgs& a, const TcUnit* uni
     }
 }
 
+// A block of few rows, without TMEM: the groups take its tiles in turn and a warp 32 keys of a tile, with sums, maxima and an
+// output of its own. (All warps on every tile, 16 keys each: 10 us more at 256 sequences.)
 template <typename T, int HD>
+__device__ __forceinline__ bool few_rows(const TreeArgs& a, const TcUnit* now, unsigned units, unsigned ring_t, unsigned met, bool ok) {
+    using S = TcShape<HD>;
+    extern __shared__ __align__(1024) unsigned char tc_smem[];
+    const uint32_t smem = smem_addr(tc_smem), bars = smem + S::kBars;
+    const unsigned tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, w = warp >> 2;
+    const TcBars<HD> at_bar{bars};
+    volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(tc_smem + S::kMisc);
+    volatile int* gave_up = reinterpret_cast<volatile int*>(misc + 1);
+    float2* ml = reinterpret_cast<float2*>(tc_smem + S::kMl);
+    const float scale = a.scale_log2;
+    const auto full = [&](unsigned slot) { return at_bar.full(slot); };
+    const auto empty = [&](unsigned slot) { return at_bar.empty(slot); };
+    const uint32_t qfull = at_bar.qfull(), qfree = qfull + 16, fbar = at_bar.fbar();
+    const auto look = [&](unsigned slot, unsigned round) {
+        ok = ok && __all_sync(0xffffffffu, tc_wait(full(slot), round, a.wait_limit, gave_up));
+        if (ok && lane == 0) mbar_arrive(empty(slot));
+        __syncwarp();
+    };
+    const auto meet = [&] {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(fbar);
+        ok = __all_sync(0xffffffffu, tc_wait(fbar, met, a.wait_limit, gave_up)) && ok;
+        met ^= 1u;
+    };
+    const unsigned n = now->n, qb = units & 1u, g = lane >> 2, c = lane & 3u, pair = warp & 3u;
+    const unsigned flat0 = now->block * a.block_rows, m_rows = rows_of(a, now->drafted, now->block);
+    const int len = static_cast<int>(now->len), ctx = now->ctx();
+    const TreeSeq seq{now->row0, now->drafted, ctx, len, 0u};
+    unsigned node[2];  // of rows g and g + 8
+    unsigned long long words[2][2] = {{0ull, 0ull}, {0ull, 0ull}};
+    const bool has_mask = a.mask && static_cast<int>((now->k0 + n) * kTcKeys) > ctx;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        node[h] = (flat0 + min(g + 8 * h, m_rows - 1)) / a.group;
+        if (has_mask) {
+            const unsigned long long* mask = a.mask + static_cast<size_t>(now->row0 + node[h]) * a.mask_words;
+            words[h][0] = mask[0];
+            if (a.mask_words > 1) words[h][1] = mask[1];
+        }
+    }
+    ok = __all_sync(0xffffffffu, ok && tc_wait(qfull + 8 * qb, (units >> 1) & 1u, a.wait_limit, gave_up));
+    uint32_t q[HD / 16][4];
+#pragma unroll
+    for (int s = 0; s < HD / 16; s++) ldsm4(q[s], piece_of(smem + qb * S::kTile, lane & 15u, 2 * s + (lane >> 4)));
+    meet();  // all have the query rows: their tile is where the sums are put together
+    float o[HD / 8][4];
+#pragma unroll
+    for (int j = 0; j < HD / 8; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+    float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+    const auto look_at = [&](unsigned at) { look(at % S::kSlots, (at / S::kSlots) & 1u); };
+    for (unsigned i = 0; ok && i < n; i++) {
+        const unsigned k_at = 2 * ring_t + k_place<HD>(i), v_at = 2 * ring_t + v_place<HD>(i, n);
+        if ((ring_t + i + w) & 1u) {  // the other group's; its V is looked at with this group's next
+            look_at(k_at);
+            if (i + 1 == n) look_at(v_at);
+            continue;
+        }
+        const unsigned k_slot = k_at % S::kSlots, v_slot = v_at % S::kSlots;
+        const uint32_t k_tile = smem + S::kRing + k_slot * S::kTile, v_tile = smem + S::kRing + v_slot * S::kTile;
+        const int pos0 = static_cast<int>((now->k0 + i) * kTcKeys + pair * 32);
+        ok = __all_sync(0xffffffffu, tc_wait(full(k_slot), (k_at / S::kSlots) & 1u, a.wait_limit, gave_up));
+        if (!ok) break;
+        float z[4][4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) z[x][0] = z[x][1] = z[x][2] = z[x][3] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < HD / 16; s++) {
+#pragma unroll
+            for (int x = 0; x < 4; x += 2) {
+                uint32_t k[4];  // keys 0 - 7 and 8 - 15 of 16, two pieces each
+                ldsm4(k, piece_of(k_tile, pair * 32 + x * 8 + (lane >> 4) * 8 + (lane & 7u), 2 * s + ((lane >> 3) & 1u)));
+                mma16<T>(z[x], q[s], k[0], k[1]);
+                mma16<T>(z[x + 1], q[s], k[2], k[3]);
+            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty(k_slot));
+        const bool masked = pos0 + 32 > ctx;
+        if (masked) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const unsigned seen = (seq.n <= 128 ? tree_visible2(a, seq, node[h], pos0, words[h][0], words[h][1]) : tree_visible(a, seq, node[h], pos0)) >> (2 * c);
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++) z[x][2 * h + e] = (seen >> (8 * x + e)) & 1u ? z[x][2 * h + e] : -INFINITY;
+                }
+            }
+        }
+        float top[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            top[h] = fmaxf(fmaxf(fmaxf(z[0][2 * h], z[0][2 * h + 1]), fmaxf(z[1][2 * h], z[1][2 * h + 1])),
+                           fmaxf(fmaxf(z[2][2 * h], z[2][2 * h + 1]), fmaxf(z[3][2 * h], z[3][2 * h + 1])));
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+            if (top[h] != -INFINITY) top[h] *= scale;
+        }
+        if (__any_sync(0xffffffffu, top[0] > mx[0] + 8.0f || top[1] > mx[1] + 8.0f)) {
+            float f[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const float before = mx[h];
+                mx[h] = fmaxf(before, top[h]);
+                f[h] = before == -INFINITY ? 0.0f : ex2(before - mx[h]);
+                sum[h] *= f[h];
+            }
+#pragma unroll
+            for (int j = 0; j < HD / 8; j++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[j][e] *= f[e >> 1];
+            }
+        }
+        uint32_t p[2][4];  // of 16 keys: weights of keys 2c, 2c + 1 and 2c + 8, 2c + 9, rows g and g + 8
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const float ref = mx[h] == -INFINITY ? 0.0f : mx[h];
+            float part[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const float y0 = ex2(fmaf(z[x][2 * h], scale, -ref)), y1 = ex2(fmaf(z[x][2 * h + 1], scale, -ref));
+                part[x & 1] += y0 + y1;
+                p[x >> 1][2 * (x & 1) + h] = pack2<T>(y0, y1);
+            }
+            sum[h] += part[0] + part[1];
+        }
+        if (i) look_at(2 * ring_t + v_place<HD>(i - 1, n));
+        ok = __all_sync(0xffffffffu, ok && tc_wait(full(v_slot), (v_at / S::kSlots) & 1u, a.wait_limit, gave_up));
+        if (!ok) break;
+        if (masked) {
+            // as in clear_v, the warp's own 32 rows, four at a time
+            for (int r0 = max(0, ctx - pos0) & ~3; r0 < 32; r0 += 4) {
+                const int r = r0 + static_cast<int>(lane >> 3), pos = pos0 + r;
+                uint4* v = reinterpret_cast<uint4*>(tc_smem + S::kRing + v_slot * S::kTile + (pair * 32 + r) * 128) + (lane & 7u);
+#pragma unroll
+                for (int e = 0; e < S::kSubs; e++) {
+                    if (pos >= len) v[e * (S::kPanel / 16)] = make_uint4(0u, 0u, 0u, 0u);
+                    else if (pos >= ctx && make_finite<T>(v + e * (S::kPanel / 16))) misc[2 + (units & 3u)] = 1;
+                }
+            }
+            proxy_fence();
+            __syncwarp();
+        }
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+#pragma unroll
+            for (int j = 0; j < HD / 16; j++) {
+                uint32_t v[4];  // columns 16 j .. + 7 and + 8 .. + 15, keys 0 - 7 and 8 - 15 each
+                ldsm4_t(v, piece_of(v_tile, pair * 32 + x * 16 + (lane & 15u), 2 * j + (lane >> 4)));
+                mma16<T>(o[2 * j], p[x], v[0], v[1]);
+                mma16<T>(o[2 * j + 1], p[x], v[2], v[3]);
+            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty(v_slot));
+    }
+    // Eight warps' sums to four (warps 4 - 7 leave theirs for warps 0 - 3), then all threads put the four together.
+    float* all = reinterpret_cast<float*>(tc_smem + qb * S::kTile);  // [4][16 rows][HD], the columns turned by the row
+    const auto place_of = [&](unsigned from, unsigned row, unsigned col) { return (from * 16 + row) * HD + (col ^ ((row & 3u) << 3)); };
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+    }
+    const auto leave = [&] {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            if (c == 0) ml[pair * 16 + g + 8 * h] = make_float2(mx[h], sum[h]);
+#pragma unroll
+            for (int j = 0; j < HD / 8; j++) *reinterpret_cast<float2*>(all + place_of(pair, g + 8 * h, 8 * j + 2 * c)) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
+        }
+    };
+    if (warp >= 4) leave();
+    meet();
+    const bool fix = misc[2 + (units & 3u)] != 0;
+    if (tid == 0) misc[2 + ((units + 2) & 3u)] = 0;
+    if (warp < 4) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const float2 other = ml[pair * 16 + g + 8 * h];
+            const float both = fmaxf(mx[h], other.x), ref = both == -INFINITY ? 0.0f : both;
+            const float f_own = sum[h] == 0.0f ? 0.0f : ex2(mx[h] - ref), f_other = other.y == 0.0f ? 0.0f : ex2(other.x - ref);
+#pragma unroll
+            for (int j = 0; j < HD / 8; j++) {
+                const float2 x = *reinterpret_cast<const float2*>(all + place_of(pair, g + 8 * h, 8 * j + 2 * c));
+                o[j][2 * h] = fmaf(o[j][2 * h], f_own, x.x * f_other);
+                o[j][2 * h + 1] = fmaf(o[j][2 * h + 1], f_own, x.y * f_other);
+            }
+            sum[h] = fmaf(sum[h], f_own, other.y * f_other);
+            mx[h] = both;
+        }
+        __syncwarp();
+        leave();
+    }
+    meet();
+    const unsigned row = tid & 15u, c0 = (tid >> 4) * (HD / 16);
+    if (row < m_rows) {
+        const bool whole = (now->slot_piece & 2u) != 0;
+        float2 parts[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) parts[x] = ml[x * 16 + row];
+        const float most = fmaxf(fmaxf(parts[0].x, parts[1].x), fmaxf(parts[2].x, parts[3].x)), ref = most == -INFINITY ? 0.0f : most;
+        float total = 0.0f, f[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            f[x] = parts[x].y == 0.0f ? 0.0f : ex2(parts[x].x - ref);
+            total = fmaf(parts[x].y, f[x], total);
+        }
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        const unsigned flat = flat0 + row, node_r = flat / a.group, head = now->kv_head * a.group + flat % a.group;
+        T* out = static_cast<T*>(a.out) + static_cast<size_t>(now->row0 + node_r) * a.out_stride + static_cast<size_t>(head) * HD;
+        const unsigned piece = blockIdx.x * 2 + (now->slot_piece & 1u);
+        float* po = a.part_o + piece_at(piece, HD, 0, row);
+        float y[HD / 16];
+#pragma unroll
+        for (int e = 0; e < HD / 16; e++) y[e] = 0.0f;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+#pragma unroll
+            for (int e = 0; e < HD / 16; e += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(all + place_of(x, row, c0 + e));
+                y[e] = fmaf(v.x, f[x], y[e]);
+                y[e + 1] = fmaf(v.y, f[x], y[e + 1]);
+                y[e + 2] = fmaf(v.z, f[x], y[e + 2]);
+                y[e + 3] = fmaf(v.w, f[x], y[e + 3]);
+            }
+        }
+        if (whole) {
+#pragma unroll
+            for (int e = 0; e < HD / 16; e += 4)
+                *reinterpret_cast<uint2*>(out + c0 + e) = make_uint2(pack2<T>(y[e] * inv, y[e + 1] * inv), pack2<T>(y[e + 2] * inv, y[e + 3] * inv));
+        } else {
+#pragma unroll
+            for (int e = 0; e < HD / 16; e++) po[static_cast<size_t>(c0 + e) * kTcRows] = y[e];
+            if (c0 == 0) a.part_ml[piece * kTcRows + row] = make_float2(most, total);
+        }
+        if (fix && total != 0.0f) add_bad_values<T, HD>(a, now, node_r, head, ref, total, out, whole ? nullptr : po, c0, c0 + HD / 16);
+    }
+    proxy_fence();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(qfree + 8 * qb);
+    return ok;
+}
+
+// FEW: blocks of few rows take the products of a warp.
+template <typename T, int HD, bool FEW>
 __global__ void __launch_bounds__(kTcThreads, 1)
     tree_attn_tc_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v) {
@@ -291,13 +607,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t smem = smem_addr(tc_smem);
     const unsigned tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     const uint32_t bars = smem + S::kBars;
-    const auto full = [&](unsigned slot) { return bars + slot * 8; };
-    const auto empty = [&](unsigned slot) { return bars + (S::kSlots + slot) * 8; };
-    const auto sfull = [&](unsigned b) { return bars + (2 * S::kSlots + b) * 8; };                  // scores are there
-    const auto pready = [&](unsigned b) { return bars + (2 * S::kSlots + S::kScores + b) * 8; };    // weights are there
-    const auto sfree = [&](unsigned b) { return bars + (2 * S::kSlots + 2 * S::kScores + b) * 8; };  // weights have been used
-    const uint32_t qfull = bars + (2 * S::kSlots + 3 * S::kScores) * 8, qfree = qfull + 16, udone = qfull + 32;  // Q tiles 0 and 1 each; the last product of a block
-    const uint32_t ufull = udone + 8, fbar = ufull + 8 * S::kUnits;  // a block is described; the softmax groups meet
+    const TcBars<HD> at_bar{bars};
+    const auto full = [&](unsigned slot) { return at_bar.full(slot); };
+    const auto empty = [&](unsigned slot) { return at_bar.empty(slot); };
+    const auto sfull = [&](unsigned b) { return at_bar.sfull(b); };
+    const auto pready = [&](unsigned b) { return at_bar.pready(b); };
+    const auto sfree = [&](unsigned b) { return at_bar.sfree(b); };
+    const uint32_t qfull = at_bar.qfull(), qfree = qfull + 16, udone = at_bar.udone(), ufull = at_bar.ufull(), fbar = at_bar.fbar();
     volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(tc_smem + S::kMisc);  // [0] TMEM, [1] a wait gave up, [2..5] bad values, by block
     volatile int* gave_up = reinterpret_cast<volatile int*>(misc + 1);
     float2* ml = reinterpret_cast<float2*>(tc_smem + S::kMl);
@@ -305,14 +621,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (warp == 8) {
         tc_alloc(smem + S::kMisc, 512);
         if (lane == 0) {
-            for (unsigned i = 0; i < 2 * S::kSlots + S::kScores; i++) mbar_init(bars + i * 8, 1);
+            for (unsigned i = 0; i < 2 * S::kSlots; i++) mbar_init(bars + i * 8, FEW && i >= S::kSlots ? 10 : 1);  // full, empty
+            for (unsigned b = 0; b < S::kScores; b++) mbar_init(sfull(b), 1);
             for (unsigned b = 0; b < S::kScores; b++) {
                 mbar_init(pready(b), 4);
                 mbar_init(sfree(b), 1);
             }
             for (unsigned b = 0; b < 2; b++) {
                 mbar_init(qfull + 8 * b, 1);
-                mbar_init(qfree + 8 * b, 1);
+                mbar_init(qfree + 8 * b, FEW ? 10 : 1);
             }
             mbar_init(udone, 1);
             for (unsigned i = 0; i < S::kUnits; i++) mbar_init(ufull + 8 * i, 1);
@@ -344,6 +661,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     TreeWalk<kTcKeys> walk;
     walk.start(a, place, ok ? share.first(blockIdx.x) : 0u, ok ? share.first(blockIdx.x + 1) : 0u, known);
     TreeUnit u;
+
+    // A wait by parity cannot tell a phase from the one after the next, so a warp that waits for tiles has to have seen each
+    // place of the ring filled before it asks for the next filling. Tiles that a warp has no use for it looks on: it waits for
+    // them and counts as one of those that empty them.
+    const auto look = [&](unsigned slot, unsigned round) {
+        ok = ok && __all_sync(0xffffffffu, tc_wait(full(slot), round, a.wait_limit, gave_up));
+        if (ok && lane == 0) mbar_arrive(empty(slot));
+        __syncwarp();
+    };
+    const auto look_on = [&](RingAt<HD>& at, unsigned n) {  // a whole block of n tiles
+        for (unsigned i = 0; ok && i < n; i++) {
+            RingAt<HD> k = at, v = at;
+            k.skip(k_place<HD>(i));
+            v.skip(v_place<HD>(i, n));
+            look(k.slot, k.round);
+            look(v.slot, v.round);
+        }
+        at.skip(2 * n);
+    };
 
     if (warp == 8 || warp == 11) {
         // ---- K tiles (warp 8), query rows and V tiles (warp 11) ----
@@ -442,6 +778,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint64_t q_desc = tc_desc(smem, 16), k_desc = tc_desc(smem + S::kRing, 16);
         RingAt<HD> at;                     // of the next K tile
         unsigned b = 0, b_round = 0, t = 0, units = 0;  // S tile, key tiles, blocks
+        bool few = false;                  // the block before was one of few rows
         const auto wait = [&](uint32_t bar, unsigned parity) { ok = ok && __all_sync(0xffffffffu, tc_wait(bar, parity, a.wait_limit, gave_up)); };
         TcUnit* described = reinterpret_cast<TcUnit*>(tc_smem + S::kUnit);
         const auto publish = [&](unsigned n) {  // block `units`, to the softmax groups
@@ -455,6 +792,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const unsigned n = u.k1 - u.k0, qb = units & 1u;
             publish(n);
             wait(qfull + 8 * qb, (units >> 1) & 1u);
+            if (FEW && rows_of(a, u.seq.n, u.block) <= kFewRows) {  // the softmax groups do it all
+                if (t) wait(sfree((t - 1) % S::kScores), ((t - 1) / S::kScores) & 1u);  // all tiles so far have come, V as well
+                look_on(at, n);
+                if (ok && lane == 0) mbar_arrive(qfree + 8 * qb);
+                __syncwarp();
+                few = true;
+                units++;
+                continue;
+            }
+            // K tiles are not to be used up here while V tiles of a block of few rows still lie in the ring: the copies of K
+            // would run more than a round ahead of those of V.
+            if (FEW && few) wait(qfree + 8 * (qb ^ 1u), ((units - 1) >> 1) & 1u);
+            few = false;
             for (unsigned i = 0; ok && i < n; i++) {
                 wait(full(at.slot), at.round);
                 if (t >= S::kScores) wait(sfree(b), b_round ^ 1u);  // the weights that these scores overwrite have been used
@@ -469,7 +819,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                     tc_commit(sfull(b));
                     tc_commit(empty(at.slot));
-                    if (i == n - 1) tc_commit(qfree + 8 * qb);
+                    if (FEW) mbar_arrive_n(empty(at.slot), 9);
+                    if (i == n - 1) {
+                        tc_commit(qfree + 8 * qb);
+                        if (FEW) mbar_arrive_n(qfree + 8 * qb, 9);
+                    }
                 }
                 __syncwarp();
                 if (++b == S::kScores) {
@@ -491,10 +845,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         constexpr uint32_t idesc = tc_idesc(std::is_same<T, __half>::value ? 0u : 1u, HD, 1);
         const uint64_t v_desc = tc_desc(smem + S::kRing, S::kPanel);
         RingAt<HD> at;
-        unsigned b = 0, b_round = 0, t = 0, units = 0;
+        unsigned b = 0, b_round = 0, t = 0, units = 0, blocks = 0;  // ..., blocks with products here, all blocks
         const auto wait = [&](uint32_t bar, unsigned parity) { ok = ok && __all_sync(0xffffffffu, tc_wait(bar, parity, a.wait_limit, gave_up)); };
         while (ok && walk.next(a, u)) {
             const unsigned n = u.k1 - u.k0;
+            if (FEW && rows_of(a, u.seq.n, u.block) <= kFewRows) {
+                look_on(at, n);
+                if (ok && lane == 0) mbar_arrive(qfree + 8 * (blocks & 1u));
+                __syncwarp();
+                blocks++;
+                continue;
+            }
+            blocks++;
             unsigned begun = 0;  // bit w: stream w of the block has something in its accumulator
             unsigned behind = v_place<HD>(0, n);
             at.add(behind);
@@ -511,6 +873,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         tc_mma_ts(tmem + S::kScores * 128 + w * HD, tmem + b * 128 + k * 8, vd + k * (2048 >> 4), idesc, k != 0 || (begun >> w) & 1u);
                     tc_commit(sfree(b));
                     tc_commit(empty(at.slot));
+                    if (FEW) mbar_arrive_n(empty(at.slot), 9);
                     if (i == n - 1) tc_commit(udone);
                 }
                 __syncwarp();
@@ -537,25 +900,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t lanes = (warp & 3u) << 21;  // the warp's 32 lanes of TMEM
         const uint32_t o_at = tmem + S::kScores * 128 + lanes;
         const float scale = a.scale_log2;
-        unsigned t = 0, units = 0;  // key tiles and blocks before the block (a key tile is two of the ring's)
+        // before the block: key tiles (each is two of the ring's) and blocks, all and those with products on the big tensor cores
+        unsigned ring_t = 0, units = 0, t = 0, big_units = 0;
         const TcUnit* described = reinterpret_cast<const TcUnit*>(tc_smem + S::kUnit);
         // of the block before this one, which may not have been written yet
         float last_m = 0.0f, last_l = 0.0f;
         bool pending = false;
-        // The two groups meet, twice for every block. (A wait that can give up, not a hardware barrier: were one group to
+        // The two groups meet. (A wait that can give up, not a hardware barrier: were one group to
         // give up on something else, the other would stand there for good.)
-        const auto meet = [&](unsigned phase) {
+        unsigned met = 0;
+        const auto meet = [&](unsigned phase) {  // twice for every block, unless there are blocks of few rows
             __syncwarp();
             if (lane == 0) mbar_arrive(fbar);
-            ok = __all_sync(0xffffffffu, tc_wait(fbar, phase, a.wait_limit, gave_up)) && ok;
+            ok = __all_sync(0xffffffffu, tc_wait(fbar, FEW ? met : phase, a.wait_limit, gave_up)) && ok;
+            met ^= 1u;
         };
         // The two streams of a block are put together and written out.
         const auto finish = [&] {
             const unsigned which = units - 1;  // the block's number
             const TcUnit* last = described + which % S::kUnits;
             const bool whole = (last->slot_piece & 2u) != 0;
-            const unsigned flat0 = last->block * a.block_rows, m_rows = min(a.block_rows, last->drafted * a.group - flat0);
-            ok = __all_sync(0xffffffffu, ok && tc_wait(udone, which & 1u, a.wait_limit, gave_up));
+            const unsigned flat0 = last->block * a.block_rows, m_rows = rows_of(a, last->drafted, last->block);
+            ok = __all_sync(0xffffffffu, ok && tc_wait(udone, (FEW ? big_units - 1 : which) & 1u, a.wait_limit, gave_up));
             tc_fence_after();
             ml[w * 128 + row] = make_float2(last_m, last_l);
             meet(0);
@@ -676,11 +1042,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             tc_wait_st();
         };
-        // V rows behind the last position are cleared (they may hold anything, and 0 * NaN is NaN); so are drafted ones with an
-        // infinity or a NaN, which rows that do not see them must not get: add_bad_values.
+        // V rows behind the last position are cleared (they may hold anything, and 0 * NaN is NaN); infinities and NaNs of
+        // drafted ones become 0, as rows that do not see them must not get them: add_bad_values.
         // `helpers` threads, this one number `me` of them, share it: the warps that have no rows, or all four.
         const auto clear_v = [&](unsigned i, unsigned n, int valid, int drafted, unsigned me, unsigned helpers) {
-            const unsigned at = 2 * t + v_place<HD>(i, n), slot = at % S::kSlots;
+            const unsigned at = 2 * (FEW ? ring_t : t) + v_place<HD>(i, n), slot = at % S::kSlots;
             ok = __all_sync(0xffffffffu, ok && tc_wait(full(slot), (at / S::kSlots) & 1u, a.wait_limit, gave_up));
             if (!ok) return;
             unsigned char* v_at = tc_smem + S::kRing + slot * S::kTile;
@@ -689,27 +1055,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const unsigned r = valid + e / pieces, c = e % pieces;
                 *reinterpret_cast<uint4*>(v_at + (c / 8) * S::kPanel + r * 128 + (c % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
-            // eight threads to a panel row: a row is cleared by the threads that read it
+            // eight threads to a panel row
             const unsigned g8 = me >> 3, c8 = me & 7u;
-            for (int r0 = drafted; r0 < valid; r0 += static_cast<int>(helpers >> 3)) {
-                const int r = r0 + static_cast<int>(g8);
-                bool bad = false;
-                if (r < valid) {
+            for (int r = drafted + static_cast<int>(g8); r < valid; r += static_cast<int>(helpers >> 3)) {
 #pragma unroll
-                    for (int c = 0; c < S::kSubs; c++) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(v_at + c * S::kPanel + r * 128 + c8 * 16);
-                        bad = bad || bad_pair<T>(x.x) || bad_pair<T>(x.y) || bad_pair<T>(x.z) || bad_pair<T>(x.w);
-                    }
-                }
-                const unsigned who = __ballot_sync(0xffffffffu, bad);
-                if ((who >> (lane & 24u)) & 0xffu) {
-#pragma unroll
-                    for (int c = 0; c < S::kSubs; c++) *reinterpret_cast<uint4*>(v_at + c * S::kPanel + r * 128 + c8 * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    misc[2 + (units & 3u)] = 1;
+                for (int c = 0; c < S::kSubs; c++) {
+                    if (make_finite<T>(reinterpret_cast<uint4*>(v_at + c * S::kPanel + r * 128 + c8 * 16))) misc[2 + (units & 3u)] = 1;
                 }
             }
             proxy_fence();
         };
+        bool few = false;  // the block before was one of few rows
         if (place.seq >= a.n_seqs) ok = false;
         while (ok) {
             ok = __all_sync(0xffffffffu, tc_wait(ufull + 8 * (units % S::kUnits), (units / S::kUnits) & 1u, a.wait_limit, gave_up));
@@ -717,7 +1073,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const TcUnit* now = described + units % S::kUnits;
             const unsigned n = now->n;
             if (n == 0 && !pending) break;
-            const unsigned flat0 = now->block * a.block_rows, m_rows = min(a.block_rows, now->drafted * a.group - flat0);
+            const unsigned flat0 = now->block * a.block_rows, m_rows = rows_of(a, now->drafted, now->block);
+            if (FEW && n && m_rows <= kFewRows) {
+                if (pending) finish();
+                ok = few_rows<T, HD>(a, now, units, ring_t, met, ok);
+                met ^= 1u;  // they met three times
+                few = true;
+                ring_t += n;
+                units++;
+                continue;
+            }
+            if (FEW && few && n) meet(0);  // what the block before left in shared memory has been read
+            few = false;
             const unsigned node = (flat0 + min(row, m_rows - 1)) / a.group;
             const int pos_first = static_cast<int>(now->k0) * kTcKeys, ctx = now->ctx();
             const bool busy = (warp & 3u) * 32 < m_rows;  // some row of the warp is there
@@ -771,7 +1138,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             last_l = l;
             pending = true;
             t += n;
+            ring_t += n;
             units++;
+            big_units++;
         }
     }
     tc_fence_before();
@@ -922,7 +1291,11 @@ int launch_tc(lokal_cuda_ctx* ctx, cudaStream_t s, const TreeArgs& a) {
     if (!encode_q(&map_q, a, half) || !encode_store(&map_k, a, a.k, half) || !encode_store(&map_v, a, a.v, half))
         return ctx->fail(LOKAL_ERR_CUDA, "tree_attn: q or a store cannot be described to the copy engine");
     const unsigned shares = tc_shares(ctx);
-    launch_staged(tree_attn_tc_kernel<T, HD>, shares, kTcThreads, TcShape<HD>::kBytes, s, a, map_q, map_k, map_v);
+    // Few rows on average: the kernel that looks at each block (figures at the top).
+    if (HD == 64 && static_cast<unsigned long long>(a.rows) * a.group <= static_cast<unsigned long long>(a.n_seqs) * kFewRows)
+        launch_staged(tree_attn_tc_kernel<T, HD, HD == 64>, shares, kTcThreads, TcShape<HD>::kBytes, s, a, map_q, map_k, map_v);
+    else
+        launch_staged(tree_attn_tc_kernel<T, HD, false>, shares, kTcThreads, TcShape<HD>::kBytes, s, a, map_q, map_k, map_v);
     LOKAL_CHECK_LAUNCH(ctx, "tree_attn_tc_kernel");
     launch_k(tree_join_tc_kernel<T>, dim3(shares - 1, 8), 256, 0, s, a, shares);
     LOKAL_CHECK_LAUNCH(ctx, "tree_join_tc_kernel");

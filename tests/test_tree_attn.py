@@ -614,3 +614,61 @@ def test_the_same_bits_every_time(ctx, dev, dtype, kv, hd):
         c.call()
         ctx.stream_sync()
         assert np.array_equal(dev.get(c.d["out"]), first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("mask", ["tree", "random", None])
+def test_sequences_of_few_rows_beside_some_of_many(ctx, dev, dtype, mask):
+    """Head size 64 with few rows to a sequence on average: blocks of up to 16 rows and larger ones (and the short last block of a
+    long sequence), in any order, of one key tile and of many."""
+    rng = np.random.default_rng(113)
+    drafts = rng.integers(0, 8, 40)
+    drafts[[3, 4, 17, 30]] = [65, 40, 70, 9]
+    lens = drafts + rng.choice([0, 1, 90, 128, 700, 2500], 40)
+    lens[drafts == 0] += 1
+    assert drafts.sum() * 2 <= 16 * 40
+    c = Case(ctx, dev, lens=lens, drafts=drafts, hq=6, hkv=3, hd=64, dtype=dtype, kv=dtype, mask=mask, seed=114)
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 4, 64), (32, 2, 64), (2, 2, 64), (8, 4, 128)])
+def test_single_tokens_of_many_long_sequences(ctx, dev, hq, hkv, hd):
+    rng = np.random.default_rng(115)
+    n = 96
+    c = Case(ctx, dev, lens=rng.integers(1, 4000, n), drafts=np.ones(n, np.int64), hq=hq, hkv=hkv, hd=hd, dtype=BF16, kv=BF16, mask=None, seed=116)
+    first = c.run()
+    c.check(first)
+    for _ in range(5):
+        assert np.array_equal(c.run(), first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv,hd", [(F16, F16, 64), (BF16, BF16, 64), (F16, F16, 128), (F32, F16, 64)])
+def test_what_few_rows_do_not_see_does_not_reach_them(ctx, dev, dtype, kv, hd):
+    """As above with short sequences, where the rows that see a bad value would show the loss of the key's other columns."""
+    c = Case(ctx, dev, lens=[150, 8, 131], drafts=[6, 8, 5], hq=4, hkv=2, hd=hd, dtype=dtype, kv=kv, mask="tree", seed=117)
+    clean = c.run()
+    c.check(clean)
+    used = np.zeros(c.n_pages * c.page, bool)
+    for i in range(3):
+        used[c.cache_row(i, np.arange(int(c.lens[i])))] = True
+    c.k[~used], c.v[~used] = np.nan, np.inf
+    assert np.array_equal(c.run(), clean), "rows that belong to nobody"
+    for i, node, bad in [(0, 2, np.nan), (1, 3, np.inf), (2, 3, -np.inf)]:
+        row = c.cache_row(i, np.array([int(c.lens[i] - c.drafts[i]) + node]))[0]
+        before = c.v[row].copy()
+        c.v[row, 3::hd] = bad
+        got = c.run()
+        c.v[row] = before
+        r0, n = int(c.starts[i]), int(c.drafts[i])
+        rows = np.zeros(c.rows, bool)
+        rows[r0:r0 + n] = visible(n, 0, c.mask[r0:r0 + n])[:, node]
+        good = got.copy()
+        good[rows] = clean[rows]
+        c.check(good, f"bad row {node} of sequence {i}")
+        hit, was = got[rows].reshape(-1, c.hq, hd), clean[rows].reshape(-1, c.hq, hd)
+        assert rows.any() and not np.isfinite(hit[:, :, 3]).any()
+        # two results of the same formula, each within its tolerance (values of order 1): 2 * 2^-8 of the largest, and to spare
+        assert np.allclose(np.delete(hit, 3, axis=2), np.delete(was, 3, axis=2), rtol=0.05, atol=0.05)
