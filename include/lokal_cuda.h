@@ -427,7 +427,7 @@ LOKAL_API int lokal_cuda_kv_pool_accept(lokal_cuda_ctx* ctx, lokal_cuda_stream s
  * (speculative decoding); one row per sequence is plain decoding, a chain is a causal chunk.
  *
  * Sequence i has rows [q_start[i], q_start[i + 1]) of the call (device int32[n_seqs + 1]; rows of the call that belong to
- * no sequence are neither read nor written) and is slot slots[i] (slot i with slots NULL). Its n rows are the LAST n of
+ * no sequence have no effect and are not written) and is slot slots[i] (slot i with slots NULL). Its n rows are the LAST n of
  * the slot's positions: reserve them, stage their K and V (lokal_cuda_kv_stage, lokal_cuda_qk_rope with k_out_rows), then
  * attend. The c = lens[slot] - n positions before them are committed.
  *
@@ -450,8 +450,9 @@ LOKAL_API size_t lokal_cuda_tree_attn_workspace(const lokal_cuda_ctx* ctx, size_
  * infinities and NaN included, and rows of a page behind the slot's last position may hold anything.
  * k_store, v_store: numbers of the pool's stores; their rows start with n_kv_heads * head_dim elements of kv_dtype.
  * q, out: [rows][n_q_heads * head_dim] of dtype at the given row strides (elements); out must not overlap q.
- * Types F32 / F16 / BF16, any of them for either; scores, maxima and sums are f32, and so are the products unless q and
- * the cache have the same 16-bit type, where the tensor cores take the weights rounded to that type. head_dim up to 256.
+ * Types F32 / F16 / BF16, any of them for either; scores, maxima and sums are f32. Where q and the cache have the same
+ * 16-bit type, the weights are rounded to it for their product with V; every other pair has the accuracy of f32 products.
+ * head_dim up to 256.
  * workspace: device memory, 16-byte aligned, of lokal_cuda_tree_attn_workspace bytes, used until the call is done: calls
  * that may overlap need one each. Nothing of it has to be kept or cleared between calls. */
 LOKAL_API int lokal_cuda_tree_attn(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const lokal_kv_pool* pool, uint32_t k_store, uint32_t v_store,

@@ -2,7 +2,7 @@
 // type, 16-bit ones over a cache of another type; head sizes 64 and 128.
 //
 // tf32 products take 11 significant bits of each factor. A value of f16 or bf16 has no more; an f32 value is split into
-// two parts, x = hi + lo with hi the upper 11 bits and lo the next 11, and a product into hi*hi + hi*lo + lo*hi (what is
+// two parts, x = hi + lo with hi x rounded to 11 bits and lo the rest rounded to 11, and a product into hi*hi + hi*lo + lo*hi (what is
 // left out is below 2^-22 of it; a factor that needs no split drops its term). So the weights, which stay f32, and the
 // query rows cost two products a piece over a 16-bit cache and three over an f32 one. Sums over the keys are taken per
 // step of 8 or 16 keys in the tensor core and joined in f32 on the outside.
