@@ -378,9 +378,10 @@ LOKAL_API int lokal_cuda_kv_stage(lokal_cuda_ctx* ctx, lokal_cuda_stream s, cons
  * or named by an earlier entry, a length the table cannot hold, no free page) is left undone, the others are not, and
  * the next lokal_cuda_stream_sync returns LOKAL_ERR_PAGE_RANGE or LOKAL_ERR_NO_PAGES.
  *
- * page_rows: a power of two, 8 to 256. n_pages * page_rows and max_pages * page_rows at most 2^31 - 1. row_bytes even;
+ * page_rows: a power of two, 8 to 256. n_pages * page_rows at most 2^31 - 1, max_pages * page_rows at most 2^31 - 256. row_bytes even;
  * with stores and row_bytes multiples of 16 bytes, copies use 16-byte accesses. A list has at most n_slots entries
- * (and 65535). `stores` is a host array of device addresses. create and destroy allocate and free: not during a capture. */
+ * (and 65535). `stores` is a host array of device addresses. create and destroy allocate and free: not during a
+ * capture, and a pool goes before its context. */
 typedef struct lokal_kv_pool lokal_kv_pool;
 LOKAL_API int lokal_cuda_kv_pool_create(lokal_cuda_ctx* ctx, uint32_t page_rows, uint32_t n_pages, uint32_t n_slots, uint32_t max_pages,
                                         int32_t* table, int32_t* lens, int32_t* refs, void* const* stores, uint32_t n_stores,
@@ -416,7 +417,9 @@ LOKAL_API int lokal_cuda_kv_pool_copy_pages(lokal_cuda_ctx* ctx, lokal_cuda_stre
 /* After drafted rows have been verified (see lokal_cuda_tree_attn: the last q_start[i + 1] - q_start[i] positions of slot
  * slots[i], or slot i with slots NULL): the rows of the accepted path, accepted[i][0 .. n_accepted[i]) in ascending
  * order, move up behind the committed ones in every store, and the slot is cut behind them. accepted is
- * [n_seqs][max_accept], max_accept at most 256. A sequence with a bad list is left as it was. */
+ * [n_seqs][max_accept], max_accept at most 256. A sequence with a bad list is left as it was. Rows move within the pages
+ * that hold them, so drafted rows have to be the slot's own: fork a slot before its drafts are reserved or after they are
+ * accepted, not between. */
 LOKAL_API int lokal_cuda_kv_pool_accept(lokal_cuda_ctx* ctx, lokal_cuda_stream s, lokal_kv_pool* pool, const uint32_t* slots,
                                         const int32_t* q_start, const int32_t* accepted, const int32_t* n_accepted, uint32_t max_accept,
                                         size_t n_seqs);

@@ -584,8 +584,8 @@ int lokal_cuda_kv_pool_create(lokal_cuda_ctx* ctx, uint32_t page_rows, uint32_t 
     if (page_rows < 8 || page_rows > 256 || (page_rows & (page_rows - 1)))
         return ctx->fail(LOKAL_ERR_BAD_ARG, "kv_pool_create: page_rows %u is not a power of two from 8 to 256", page_rows);
     if (!n_pages || !n_slots || !max_pages || !n_stores) return ctx->fail(LOKAL_ERR_BAD_ARG, "kv_pool_create: pages, slots, table width and stores must be non-zero");
-    if (static_cast<uint64_t>(n_pages) * page_rows > 0x7fffffffull || static_cast<uint64_t>(max_pages) * page_rows > 0x7fffffffull)
-        return ctx->fail(LOKAL_ERR_BAD_ARG, "kv_pool_create: more than 2^31 - 1 rows in a store or positions in a slot");
+    if (static_cast<uint64_t>(n_pages) * page_rows > 0x7fffffffull || static_cast<uint64_t>(max_pages) * page_rows > 0x7fffff00ull)  // a key tile behind the last position still counts in 32 bits
+        return ctx->fail(LOKAL_ERR_BAD_ARG, "kv_pool_create: more than 2^31 - 1 rows in a store or 2^31 - 256 positions in a slot");
     if (n_slots > 0x7fffffffu || n_stores > 65536) return ctx->fail(LOKAL_ERR_BAD_ARG, "kv_pool_create: too many slots or stores");
     if (row_bytes == 0 || row_bytes % 2 || row_bytes > (1u << 22)) return ctx->fail(LOKAL_ERR_BAD_ARG, "kv_pool_create: row_bytes %zu is zero, odd or above 4 MB", row_bytes);
     if (!lokal::aligned_to(table, 4) || !lokal::aligned_to(lens, 4) || !lokal::aligned_to(refs, 4))

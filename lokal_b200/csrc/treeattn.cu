@@ -386,6 +386,7 @@ int lokal_cuda_tree_attn(lokal_cuda_ctx* ctx, lokal_cuda_stream s, const lokal_k
     if (mask && mask_words == 0) return ctx->fail(LOKAL_ERR_BAD_ARG, "tree_attn: a mask needs mask_words");
     if (n_seqs == 0 || rows == 0) return LOKAL_OK;
     if (!q || !out || !q_start) return ctx->fail(LOKAL_ERR_BAD_ARG, "tree_attn: q, out and q_start must be non-null");
+    if (q == out) return ctx->fail(LOKAL_ERR_BAD_ARG, "tree_attn: out must not be q");
     if (q_row_stride < width || out_row_stride < width) return ctx->fail(LOKAL_ERR_BAD_ARG, "tree_attn: a row stride is smaller than the heads");
     if (!lokal::aligned_to(q, es) || !lokal::aligned_to(out, es) || !lokal::aligned_to(pool->stores[k_store], ks) || !lokal::aligned_to(pool->stores[v_store], ks) ||
         !lokal::aligned_to(q_start, 4) || !lokal::aligned_to(slots, 4) || !lokal::aligned_to(mask, 8) || !lokal::aligned_to(workspace, 16))

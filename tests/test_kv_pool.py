@@ -287,3 +287,15 @@ def test_create_refusals(ctx, dev):
     pool.fork(None, None, n=0)
     ctx.stream_sync()
     pool.close()
+
+
+@pytest.mark.gpu
+def test_the_longest_slot_leaves_room_for_a_tile(ctx, dev):
+    import torch
+    t = torch.zeros(4096, dtype=torch.int32, device="cuda")
+    good = dict(page_rows=16, n_pages=4, n_slots=2, table=t, lens=t[64:], refs=t[128:], stores=[t[256:]], row_bytes=16)
+    most = (2 ** 31 - 256) // 16
+    L.KvPool(ctx, max_pages=most, **good).close()
+    with pytest.raises(L.LokalCudaError) as e:
+        L.KvPool(ctx, max_pages=most + 1, **good)
+    assert e.value.status == capi.ERR_BAD_ARG

@@ -672,3 +672,13 @@ def test_what_few_rows_do_not_see_does_not_reach_them(ctx, dev, dtype, kv, hd):
         assert rows.any() and not np.isfinite(hit[:, :, 3]).any()
         # two results of the same formula, each within its tolerance (values of order 1): 2 * 2^-8 of the largest, and to spare
         assert np.allclose(np.delete(hit, 3, axis=2), np.delete(was, 3, axis=2), rtol=0.05, atol=0.05)
+
+
+@pytest.mark.gpu
+def test_out_is_not_q(ctx, dev):
+    c = Case(ctx, dev, lens=[50], drafts=[3], hq=4, hkv=2, hd=64, dtype=BF16, kv=BF16, seed=119)
+    d = c.upload()
+    d["out"] = d["q"]
+    with pytest.raises(L.LokalCudaError) as e:
+        c.call()
+    assert e.value.status == capi.ERR_BAD_ARG
