@@ -418,8 +418,16 @@ __global__ void __launch_bounds__(256) pool_accept_kernel(const PoolArgs a, cons
     const unsigned i = blockIdx.y;
     const unsigned slot = t.slots ? t.slots[i] : i;
     const PoolWork w = pool_work(a.work, a.n_pages, a.n_slots);
+    // A slot that an earlier sequence of the list names too is that sequence's, which may be cutting it meanwhile: the CTA
+    // leaves as a whole before it reads anything of the slot. (Were a part of its threads to see the length of before and a
+    // part that of after, some would go on with rows that nobody has worked out.)
+    bool taken = false;
+    for (unsigned k = threadIdx.x; k < i; k += 256) taken = taken || (t.slots ? t.slots[k] : k) == slot;
     if (threadIdx.x == 0) bad = 0;
-    __syncthreads();
+    if (__syncthreads_or(taken)) {
+        if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.err_word, kErrPageRange);
+        return;
+    }
     const int drafts = t.q_start[i + 1] - t.q_start[i], count = t.counts[i];
     int len = 0, base = 0;
     bool ok = slot < a.n_slots && drafts >= 0 && count >= 0 && count <= drafts && count <= static_cast<int>(t.max_accept);
@@ -446,9 +454,6 @@ __global__ void __launch_bounds__(256) pool_accept_kernel(const PoolArgs a, cons
             from[j] = (ps << a.page_shift) + ((base + x) & m);
             to[j] = (pd << a.page_shift) + ((base + j) & m);
         }
-        // a slot that an earlier sequence of the list names too is that sequence's
-        for (unsigned k = threadIdx.x; k < i; k += 256)
-            if ((t.slots ? t.slots[k] : k) == slot) bad = 1;
     }
     __syncthreads();
     ok = ok && !bad;

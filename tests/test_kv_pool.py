@@ -299,3 +299,22 @@ def test_the_longest_slot_leaves_room_for_a_tile(ctx, dev):
     with pytest.raises(L.LokalCudaError) as e:
         L.KvPool(ctx, max_pages=most + 1, **good)
     assert e.value.status == capi.ERR_BAD_ARG
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page,n_stores,width", [(16, 6, 512), (8, 2, 5)])
+def test_a_slot_that_accept_names_many_times_belongs_to_the_first(ctx, dev, page, n_stores, width):
+    """The later entries find the slot while the first one cuts it: behind the cut its length is shorter than their drafts."""
+    r = Rig(ctx, dev, page, 600, 48, 24, n_stores, width, 23)
+    rng = np.random.default_rng(23)
+    for step in range(25):
+        slots = rng.integers(0, 6, 48)
+        grow = rng.integers(20, 60, 6)
+        r.both("reserve", np.arange(6), r.m.lens[:6] + grow)
+        n = grow[slots]
+        counts = np.array([int(rng.integers(0, 9)) for _ in slots])
+        acc = np.stack([np.sort(rng.permutation(k)[:8]) for k in n])
+        r.accept(slots, n, acc, counts)
+        r.same(f"step {step}")
+        r.both("truncate", np.arange(6), rng.integers(0, 30, 6))
+        r.same(f"cut {step}")
