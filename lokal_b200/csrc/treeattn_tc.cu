@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (warp == 9 && lane < 3) tma_prefetch(lane == 0 ? &map_q : lane == 1 ? &map_k : &map_v);
     pdl_wait();
     pdl_launch();  // only now: tree_join_tc_kernel looks at the lengths before it waits for this launch
-    // the ring is not in use yet: its first bytes hold the sums of the walk
+    // the tile of the first query rows is not in use yet: its first bytes hold the sums of the walk
     const unsigned shares = gridDim.x;
     const TreePlace place = tree_locate<kTcKeys, kTcThreads>(a, reinterpret_cast<unsigned long long*>(tc_smem), blockIdx.x == 0, [&](unsigned total) {
         const TreeShares s(total, shares);
@@ -652,6 +652,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const TreeSeq q = tree_seq(a, place.seq + lane, false);
         known[lane] = make_int4(static_cast<int>(q.row0), static_cast<int>(q.n), q.len, static_cast<int>(q.slot));
     }
+    proxy_fence();  // the walk's reads and writes of the tile come before those of the copy engine
     tc_fence_before();
     __syncthreads();
     tc_fence_after();

@@ -682,3 +682,21 @@ def test_out_is_not_q(ctx, dev):
     with pytest.raises(L.LokalCudaError) as e:
         c.call()
     assert e.value.status == capi.ERR_BAD_ARG
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,drafts,hd", [(BF16, 1, 64), (F16, 40, 64), (BF16, 1, 128)])
+def test_the_first_query_rows_of_a_cta_come_through_whole(ctx, dev, dtype, drafts, hd):
+    """The tile they are copied into is where the walk to a CTA's share keeps its sums before: two calls in turn, many times, with
+    other query rows and so another walk's sums under them."""
+    n = 300
+    cases = [Case(ctx, dev, lens=np.full(n, 150 + 60 * i), drafts=np.full(n, drafts), hq=4, hkv=2, hd=hd, dtype=dtype, kv=dtype, mask=None, seed=121 + i) for i in range(2)]
+    first = [c.run() for c in cases]
+    for c, got in zip(cases, first):
+        c.check(got)
+    for _ in range(100):
+        for c in cases:
+            c.call()
+    ctx.stream_sync()
+    for c, got in zip(cases, first):
+        assert np.array_equal(dev.get(c.d["out"]), got)
