@@ -608,8 +608,11 @@ int lokal_cuda_kv_pool_create(lokal_cuda_ctx* ctx, uint32_t page_rows, uint32_t 
     void* dev = nullptr;
     cudaError_t e = p->stores ? cudaSuccess : cudaErrorMemoryAllocation;
     if (e == cudaSuccess) e = cudaMalloc(&dev, n_stores * sizeof(void*) + ints * sizeof(int));
-    if (e == cudaSuccess) e = cudaMemset(dev, 0, n_stores * sizeof(void*) + ints * sizeof(int));
-    if (e == cudaSuccess) e = cudaMemcpy(dev, stores, n_stores * sizeof(void*), cudaMemcpyHostToDevice);
+    // waited for: a copy from pageable memory returns before it has arrived, and the streams of the calls to come do not
+    // order themselves behind the default stream
+    if (e == cudaSuccess) e = cudaMemsetAsync(dev, 0, n_stores * sizeof(void*) + ints * sizeof(int), ctx->host_stream);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(dev, stores, n_stores * sizeof(void*), cudaMemcpyHostToDevice, ctx->host_stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->host_stream);
     if (e != cudaSuccess) {
         if (dev) cudaFree(dev);
         delete p;

@@ -318,3 +318,28 @@ def test_a_slot_that_accept_names_many_times_belongs_to_the_first(ctx, dev, page
         r.same(f"step {step}")
         r.both("truncate", np.arange(6), rng.integers(0, 30, 6))
         r.same(f"cut {step}")
+
+
+@pytest.mark.gpu
+def test_a_new_pool_is_ready_on_any_stream(ctx, dev):
+    """The first call on a pool is a fork on a stream that does not order itself behind the default one: it reads the addresses
+    of the stores that create has sent to the device."""
+    import torch
+    page, n_stores = 8, 300
+    s = ctx.stream_create()
+    for step in range(40):
+        store = torch.full((n_stores, 8 * page, 8), step, dtype=torch.int16, device="cuda")
+        store[:, 2 * page:] = -1
+        table = torch.tensor([[0, 1], [-1, -1]], dtype=torch.int32, device="cuda")
+        lens = torch.tensor([13, 0], dtype=torch.int32, device="cuda")
+        refs = torch.tensor([1, 1, 0, 0, 0, 0, 0, 0], dtype=torch.int32, device="cuda")
+        src, dst = (torch.tensor([i], dtype=torch.int32, device="cuda") for i in (0, 1))
+        torch.cuda.synchronize()
+        pool = L.KvPool(ctx, page_rows=page, n_pages=8, n_slots=2, max_pages=2, table=table, lens=lens, refs=refs,
+                        stores=[store[i] for i in range(n_stores)], row_bytes=16)
+        pool.fork(src, dst, n=1, stream=s)
+        ctx.stream_sync(s)
+        assert table[1].tolist() == [0, 2] and refs.tolist()[:3] == [2, 1, 1]
+        assert (store[:, 2 * page:2 * page + 5] == step).all() and (store[:, 2 * page + 5:] == -1).all()
+        pool.close()
+    ctx.stream_destroy(s)
