@@ -7,6 +7,12 @@
 // query rows cost two products a piece over a 16-bit cache and three over an f32 one. Sums over the keys are taken per
 // step of 8 or 16 keys in the tensor core and joined in f32 on the outside.
 //
+// An infinity does not survive the split (inf - inf is NaN, and an infinity times the parts of a factor has either sign), nor
+// do the largest f32 values, which round up to one. Wherever that happens to what a row sees, the row's sums are not finite. So
+// a warp that ends a block with such sums goes through its keys again, with care: scores that are not finite are summed as
+// plain f32 products, and such values of V are left out of the product and added one by one. (With care from the first, always:
+// 16 sequences of 20,000 keys, 4 rows each, 16 / 8 heads of 128, f32 over f16 took 554 us, and 472 so.)
+//
 // Bound by memory at few rows (a step of 16 keys of 128 columns is 8 KB of f16 cache and 128 products of 16 x 8 x 8).
 // Every warp is on its own: it walks every fourth run of keys of the CTA's tiles, fetches K and V from the pages straight
 // into the registers in which the product wants them, and the next K while it weighs this one; eight warps to an SM keep
@@ -32,6 +38,29 @@ __device__ __forceinline__ uint32_t tf32_round(float x) {
 }
 __device__ __forceinline__ uint32_t tf32_hi(float x) { return tf32_round(x); }
 __device__ __forceinline__ uint32_t tf32_lo(float x, uint32_t hi) { return tf32_round(x - __uint_as_float(hi)); }
+
+// Whether a value of type T goes into the product: finite, and so when it is rounded to 11 bits.
+constexpr float kTf32Over = 1.0009765625f;  // 1 + 2^-10: at least a step of tf32
+template <typename T>
+__device__ __forceinline__ bool tf32_holds(float x) { return isfinite(Split<T>::value ? x * kTf32Over : x); }
+// The same of a whole word of a run, many of them in a sum: adds 0 to t, or NaN if a value does not go into the product.
+template <typename T>
+__device__ __forceinline__ uint32_t run_word(uint32_t w, uint32_t t);
+template <>
+__device__ __forceinline__ uint32_t run_word<float>(uint32_t w, uint32_t t) { return __float_as_uint(fmaf(__uint_as_float(w) * kTf32Over, 0.0f, __uint_as_float(t))); }
+template <>
+__device__ __forceinline__ uint32_t run_word<__half>(uint32_t w, uint32_t t) {
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&w), __floats2half2_rn(0.0f, 0.0f), *reinterpret_cast<const __half2*>(&t));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <>
+__device__ __forceinline__ uint32_t run_word<__nv_bfloat16>(uint32_t w, uint32_t t) {
+    const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w), __floats2bfloat162_rn(0.0f, 0.0f), *reinterpret_cast<const __nv_bfloat162*>(&t));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// whether t, a sum of zeros of either sign, has become NaN (in either half)
+template <typename T>
+__device__ __forceinline__ bool run_odd(uint32_t t) { return (t & (Split<T>::value ? 0x7fffffffu : 0x7fff7fffu)) != 0u; }
 
 // c += a b over a contraction of 8: a 16 x 8, b 8 x 8
 __device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -153,7 +182,24 @@ __global__ void __launch_bounds__(kMmaThreads, HD == 64 ? 4 : 2) tree_attn_mma_k
             }
         };
         if (pos < pos_end) load_k(rows_now);
-        for (; pos < pos_end; pos += 4 * kStep) {
+        bool careful = false;
+        for (;; pos += 4 * kStep) {
+            if (pos >= pos_end) {
+                if (careful) break;
+                float zero = l[0] * 0.0f + l[1] * 0.0f;
+#pragma unroll
+                for (int j = 0; j < HD / 8; j++) zero += (o[j][0] * 0.0f + o[j][1] * 0.0f) + (o[j][2] * 0.0f + o[j][3] * 0.0f);
+                if (__all_sync(0xffffffffu, zero == 0.0f)) break;
+                careful = true;
+#pragma unroll
+                for (int j = 0; j < HD / 8; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+                m[0] = m[1] = -INFINITY;
+                l[0] = l[1] = 0.0f;
+                pos = u.k0 * kMmaKeys + warp * kStep;
+                rows_now = row_at(pos);
+                rows_next = row_at(pos + 4 * kStep);
+                load_k(rows_now);
+            }
             // V of the step: keys 2c and 2c + 1 of each group of 8, columns (HD / 8) g and on
             Run32 vr[NT][2][VR];
 #pragma unroll
@@ -195,6 +241,23 @@ __global__ void __launch_bounds__(kMmaThreads, HD == 64 ? 4 : 2) tree_attn_mma_k
             for (int n = 0; n < NT; n++) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) z[n][i] = CH == 4 ? (zs[0][n][i] + zs[1][n][i]) + (zs[2 % CH][n][i] + zs[3 % CH][n][i]) : zs[0][n][i] + zs[1][n][i];
+            }
+            if ((SQ || SK) && careful) {
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const unsigned row = __shfl_sync(0xffffffffu, rows_now, n * 8 + 2 * c + (i & 1));
+                        if (isfinite(z[n][i])) continue;
+                        const unsigned flat = flat0 + min(g + 8 * (i >> 1), m_rows - 1), node = flat / a.group, head = u.kv_head * a.group + flat % a.group;
+                        const TQ* q = static_cast<const TQ*>(a.q) + static_cast<size_t>(u.seq.row0 + node) * a.q_stride + static_cast<size_t>(head) * HD;
+                        const TK* k = reinterpret_cast<const TK*>(a.k + row * a.row_bytes) + static_cast<size_t>(u.kv_head) * HD;
+                        float sum = 0.0f;
+#pragma unroll 1
+                        for (int d = 0; d < HD; d++) sum = fmaf(to_f32<TQ>(q[d]), to_f32<TK>(k[d]), sum);
+                        z[n][i] = sum;
+                    }
+                }
             }
             const unsigned next = pos + 4 * kStep;
             if (next < pos_end) {
@@ -245,45 +308,57 @@ __global__ void __launch_bounds__(kMmaThreads, HD == 64 ? 4 : 2) tree_attn_mma_k
                 }
                 l[h] = fmaf(l[h], scale[h], sum);  // of this thread's keys; the four threads of a row are added at the end
             }
-            // Drafted rows with an infinity or a NaN must not reach the rows that do not see them, as 0 times it would be: they are
-            // taken out of the product and added one by one.
-            bool bad = false;
-            if (masked) {
+            // Values of V that do not go into the product are taken out of it and added one by one; where there are drafted rows,
+            // the first time through as well: they would reach the rows that do not see them, as 0 times an infinity.
+            if (pos + kStep > pos_end) {
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        bool b = false;
-                        if (pos + n * 8 + 2 * c + h >= pos_end) {
-#pragma unroll
-                            for (int r = 0; r < VR; r++) {
-#pragma unroll
-                                for (int e = 0; e < 8; e++) vr[n][h][r].w[e] = 0u;
-                            }
-                        }
+                        if (pos + n * 8 + 2 * c + h < pos_end) continue;
 #pragma unroll
                         for (int r = 0; r < VR; r++) {
 #pragma unroll
-                            for (int e = 0; e < E; e++) b = b || !isfinite(elem<TK>(vr[n][h][r], e));
-                        }
-                        if (b && static_cast<int>(pos + n * 8 + 2 * c + h) >= u.seq.ctx) {
-                            bad = true;
-#pragma unroll
-                            for (int r = 0; r < VR; r++) {
-#pragma unroll
-                                for (int e = 0; e < 8; e++)
-                                    if (sizeof(TK) == 4) {
-                                        if (!isfinite(elem<TK>(vr[n][h][r], e))) vr[n][h][r].w[e] = 0u;
-                                    } else {
-                                        if (!isfinite(elem<TK>(vr[n][h][r], (2 * e) % E))) vr[n][h][r].w[e] &= 0xffff0000u;
-                                        if (!isfinite(elem<TK>(vr[n][h][r], (2 * e + 1) % E))) vr[n][h][r].w[e] &= 0x0000ffffu;
-                                    }
-                            }
+                            for (int e = 0; e < 8; e++) vr[n][h][r].w[e] = 0u;
                         }
                     }
                 }
             }
-            bad = __any_sync(0xffffffffu, bad);
+            bool bad = false;
+            if (masked || careful) {
+                uint32_t zeros[2] = {0u, 0u};
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+#pragma unroll
+                        for (int r = 0; r < VR; r++) {
+#pragma unroll
+                            for (int e = 0; e < (HD / 8 < E ? 4 : 8); e++) zeros[h] = run_word<TK>(vr[n][h][r].w[e], zeros[h]);
+                        }
+                    }
+                }
+                bad = __any_sync(0xffffffffu, run_odd<TK>(zeros[0]) || run_odd<TK>(zeros[1]));
+            }
+            if (bad) {
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+#pragma unroll
+                        for (int r = 0; r < VR; r++) {
+#pragma unroll
+                            for (int e = 0; e < 8; e++)
+                                if (sizeof(TK) == 4) {
+                                    if (!tf32_holds<TK>(elem<TK>(vr[n][h][r], e))) vr[n][h][r].w[e] = 0u;
+                                } else {
+                                    if (!tf32_holds<TK>(elem<TK>(vr[n][h][r], (2 * e) % E))) vr[n][h][r].w[e] &= 0xffff0000u;
+                                    if (!tf32_holds<TK>(elem<TK>(vr[n][h][r], (2 * e + 1) % E))) vr[n][h][r].w[e] &= 0x0000ffffu;
+                                }
+                        }
+                    }
+                }
+            }
             // O = O * scale + P V: column 2c + e of product j is column (HD / 8) (2c + e) + j of the row
             uint32_t p_hi[NT][4], p_lo[NT][4];
 #pragma unroll
@@ -326,7 +401,7 @@ __global__ void __launch_bounds__(kMmaThreads, HD == 64 ? 4 : 2) tree_attn_mma_k
                         sees[h] = __shfl_sync(0xffffffffu, (seen[h] >> (8 * (key / 8) + key % 2)) & 1u, from);
                     }
                     const unsigned p = pos + key;
-                    if (static_cast<int>(p) < u.seq.ctx || p >= pos_end) continue;
+                    if (p >= pos_end) continue;
                     const size_t row = (static_cast<size_t>(tree_page(a, u.seq.slot, p >> a.page_shift)) << a.page_shift) + (p & (a.page_rows - 1));
                     const TK* v = reinterpret_cast<const TK*>(a.v + row * a.row_bytes) + static_cast<size_t>(u.kv_head) * HD;
 #pragma unroll
@@ -334,7 +409,7 @@ __global__ void __launch_bounds__(kMmaThreads, HD == 64 ? 4 : 2) tree_attn_mma_k
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             const float x = to_f32<TK>(v[(HD / 8) * (2 * c + e) + j]);
-                            if (isfinite(x)) continue;
+                            if (tf32_holds<TK>(x)) continue;
                             if (sees[0]) o[j][e] += w[0] * x;
                             if (sees[1]) o[j][2 + e] += w[1] * x;
                         }

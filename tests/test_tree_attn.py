@@ -700,3 +700,96 @@ def test_the_first_query_rows_of_a_cta_come_through_whole(ctx, dev, dtype, draft
     ctx.stream_sync()
     for c, got in zip(cases, first):
         assert np.array_equal(dev.get(c.d["out"]), got)
+
+
+# ---- infinities and the largest numbers in what is seen ----
+
+def seen_by(c, i):
+    n, length = int(c.drafts[i]), int(c.lens[i])
+    r0 = int(c.starts[i])
+    return visible(n, length - n, None if c.mask is None else c.mask[r0:r0 + n])
+
+
+def check_columns(c, got, columns, see, k=None, v=None):
+    """The given columns of every head against the f64 form, with `see[i]` for what the rows of sequence i see and, where given,
+    other K and V than the cache's."""
+    g, rounded = c.hq // c.hkv, c.dtype == c.kv and c.dtype != F32
+    k, v = c.k if k is None else k, c.v if v is None else v
+    for i in range(len(c.lens)):
+        n, length, r0 = int(c.drafts[i]), int(c.lens[i]), int(c.starts[i])
+        at = c.cache_row(i, np.arange(length))
+        for h in range(c.hq):
+            kc, qc = slice(h // g * c.hd, (h // g + 1) * c.hd), slice(h * c.hd, (h + 1) * c.hd)
+            out, size, terms = attention(c.q[r0:r0 + n, qc], k[at, kc], v[at, kc], see[i], np.float32(c.scale))
+            tol = tolerance(out, size, terms, length, c.hd, c.dtype, rounded)
+            bad = ~(np.abs(got[r0:r0 + n, qc] - out) <= tol)[:, columns]
+            assert not bad.any(), f"sequence {i}, head {h}: {bad.sum()} of {bad.size}"
+
+
+EVERY_PAIR = [(F32, F32, 64), (F32, F16, 64), (F32, BF16, 64), (F16, F32, 64), (F16, BF16, 64), (BF16, F16, 64), (F16, F16, 64), (BF16, BF16, 64),
+              (F32, F32, 128), (F32, F16, 128), (BF16, F32, 128), (F16, F16, 128), (BF16, BF16, 128), (F32, F16, 40), (F16, F16, 40)]
+
+
+def three_sequences(ctx, dev, dtype, kv, hd, seed):
+    return Case(ctx, dev, lens=[150, 41, 2500], drafts=[6, 9, 3], hq=4, hkv=2, hd=hd, dtype=dtype, kv=kv, seed=seed)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv,hd", EVERY_PAIR)
+def test_a_key_with_a_score_of_minus_infinity_weighs_nothing(ctx, dev, dtype, kv, hd):
+    """Committed and drafted keys with one element of -inf that all query rows meet with a positive number: exactly the result
+    without these keys."""
+    c = three_sequences(ctx, dev, dtype, kv, hd, 131)
+    column = np.abs(c.q[:, 5::hd]) + np.float32(0.25)
+    column[::2] = 1.0  # and one that any shorter type holds exactly
+    c.q[:, 5::hd] = synth.round_to(column, dtype)
+    see = [seen_by(c, i) for i in range(3)]
+    for i, pos in [(0, 3), (0, 70), (0, 146), (1, 0), (1, 33), (2, 127), (2, 128), (2, 1900), (2, 2497)]:
+        c.k[c.cache_row(i, np.array([pos]))[0], 5::hd] = -np.inf
+        see[i][:, pos] = False
+    got = c.run()
+    check_columns(c, got, np.ones(hd, bool), see, k=np.where(np.isfinite(c.k), c.k, 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv,hd", EVERY_PAIR)
+def test_an_infinite_value_in_a_committed_row_is_the_result_of_its_column(ctx, dev, dtype, kv, hd):
+    c = three_sequences(ctx, dev, dtype, kv, hd, 133)
+    for i, pos, column, value in [(0, 20, 3, np.inf), (0, 21, 9, -np.inf), (1, 31, 3, -np.inf), (2, 5, 9, np.inf), (2, 2300, 3, np.inf),
+                                  (2, 700, 20, np.inf), (2, 1500, 20, -np.inf)]:
+        c.v[c.cache_row(i, np.array([pos]))[0], column::hd] = value
+    got = c.run()
+    by_head = got[:, :c.hq * hd].reshape(-1, c.hq, hd)
+    s = [slice(int(c.starts[i]), int(c.starts[i + 1])) for i in range(3)]
+    assert (by_head[s[0], :, 3] == np.inf).all() and (by_head[s[0], :, 9] == -np.inf).all()
+    assert (by_head[s[1], :, 3] == -np.inf).all()
+    assert (by_head[s[2], :, 9] == np.inf).all() and (by_head[s[2], :, 3] == np.inf).all()
+    assert np.isnan(by_head[s[2], :, 20]).all()  # one of either sign
+    columns = np.ones(hd, bool)
+    columns[[3, 9, 20]] = False
+    see = [seen_by(c, i) for i in range(3)]
+    check_columns(c, got, columns, see, v=np.where(np.isfinite(c.v), c.v, 0))
+    for i in (0, 1):  # their other columns are as good as ever
+        assert np.isfinite(by_head[s[i]][:, :, [20] + ([9] if i else [])]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kv,hd", [(F32, F32, 64), (F32, F32, 128), (F32, F16, 64), (F32, BF16, 128), (F16, F32, 64), (BF16, F32, 128), (F32, F32, 40)])
+def test_the_largest_numbers_of_32_bits(ctx, dev, dtype, kv, hd):
+    """They round up to an infinity in shorter types. A key's meets query elements of 2e-38 (a score of some units), a query's keys of
+    0, a value's is weighed down to a finite result."""
+    most = np.finfo(np.float32).max
+    c = three_sequences(ctx, dev, dtype, kv, hd, 135)
+    if kv == F32:
+        c.q[:, 5::hd] = synth.round_to(np.full_like(c.q[:, 5::hd], 2e-38), dtype)  # 0 in f16
+        for i, pos in [(0, 10), (1, 38), (2, 2000)]:
+            c.k[c.cache_row(i, np.array([pos]))[0], 5::hd] = -most
+            c.v[c.cache_row(i, np.array([pos + 1]))[0], 7::hd] = most
+    if dtype == F32:
+        c.q[:, 11::hd] = most
+        c.k[:, 11::hd] = 0.0
+    got = c.run()
+    # a result above the largest number of a 16-bit row type is an infinity there: the column is looked at only in f32 and bf16
+    columns = np.ones(hd, bool)
+    columns[7] = dtype != F16
+    check_columns(c, got, columns, [seen_by(c, i) for i in range(3)])
