@@ -23,10 +23,12 @@
 // 181 us before, 148 so; 8 of 131,072 keys: 212 and 183 (5.9 TB/s). What it costs: blocks end slower (one key tile to a
 // sequence: 46 us before, 54), larger blocks in the same call run 6 % slower, and with head size 128, where a tile's copy takes
 // twice the time, it won 3 % at best and lost 25 % at short lengths, so those keep to the other way.
-// An accumulator is rescaled only when the maximum has grown by more than 2^8 since it was last set: weights then stay
-// below 2^8, which neither 16-bit type nor the f32 sums mind.
-// Weights are rounded to the cache's type for the product (half a step each, as the values they multiply were); sums,
-// maxima and scores are f32.
+// An accumulator is rescaled only when the maximum has grown by more than 2^lag since it was last set, so that most tiles
+// leave it alone. Weights are rounded to the cache's type for the product (half a step each, as the values they multiply
+// were); sums, maxima and scores are f32. bf16 has the exponents of f32 and takes weights of up to 2^8 and down to 2^-126. f16
+// loses bits below 2^-14, so there weights are taken times 2^11 with a lag of 2^4 (at most 2^15): half a step each down to
+// 2^-25 of the largest, and 2^-36 of it below that, where 100,000 keys of 2^-25 are 0.3 % of a row. Sums and accumulators
+// carry the factor, the division takes it out.
 #include <cuda.h>
 
 #include <type_traits>
@@ -244,6 +246,13 @@ __device__ __forceinline__ float ex2(float x) {  // 2 steps of error, 0 for resu
     return y;
 }
 
+// How far the maximum may grow before an accumulator is rescaled, and the factor of weights, as powers of 2.
+template <typename T>
+struct Weights {
+    static constexpr bool kHalf = std::is_same<T, __half>::value;
+    static constexpr float kLag = kHalf ? 4.0f : 8.0f, kUp = kHalf ? 11.0f : 0.0f;
+};
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -341,7 +350,7 @@ __device__ __noinline__ void add_bad_values(const TreeArgs& a, const TcUnit* uni
             if (!have) {
                 float s = 0.0f;
                 for (int d = 0; d < HD; d++) s = fmaf(to_f32<T>(q[d]), to_f32<T>(k[d]), s);
-                p = exp2f(fmaf(s, a.scale_log2, -m));
+                p = exp2f(fmaf(s, a.scale_log2, Weights<T>::kUp - m));
                 have = true;
             }
             if (piece) piece[static_cast<size_t>(c) * kTcRows] += p * x;
@@ -451,7 +460,7 @@ __device__ __forceinline__ bool few_rows(const TreeArgs& a, const TcUnit* now, u
             top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
             if (top[h] != -INFINITY) top[h] *= scale;
         }
-        if (__any_sync(0xffffffffu, top[0] > mx[0] + 8.0f || top[1] > mx[1] + 8.0f)) {
+        if (__any_sync(0xffffffffu, top[0] > mx[0] + Weights<T>::kLag || top[1] > mx[1] + Weights<T>::kLag)) {
             float f[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -469,7 +478,7 @@ __device__ __forceinline__ bool few_rows(const TreeArgs& a, const TcUnit* now, u
         uint32_t p[2][4];  // of 16 keys: weights of keys 2c, 2c + 1 and 2c + 8, 2c + 9, rows g and g + 8
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const float ref = mx[h] == -INFINITY ? 0.0f : mx[h];
+            const float ref = (mx[h] == -INFINITY ? 0.0f : mx[h]) - Weights<T>::kUp;
             float part[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int x = 0; x < 4; x++) {
@@ -1001,7 +1010,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             if (top != -INFINITY) top *= scale;
-            if (__any_sync(0xffffffffu, top > m + 8.0f)) {
+            if (__any_sync(0xffffffffu, top > m + Weights<T>::kLag)) {
                 const float before = m;
                 m = fmaxf(m, top);
                 const float f = before == -INFINITY ? 0.0f : ex2(before - m);
@@ -1021,7 +1030,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
             }
-            const float ref = m == -INFINITY ? 0.0f : m;
+            const float ref = (m == -INFINITY ? 0.0f : m) - Weights<T>::kUp;
             const float2 scale2 = make_float2(scale, scale), ref2 = make_float2(-ref, -ref);
             float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll

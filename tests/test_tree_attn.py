@@ -793,3 +793,41 @@ def test_the_largest_numbers_of_32_bits(ctx, dev, dtype, kv, hd):
     columns = np.ones(hd, bool)
     columns[7] = dtype != F16
     check_columns(c, got, columns, [seen_by(c, i) for i in range(3)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("drafts,hd", [(1, 64), (40, 64), (40, 128)])
+@pytest.mark.parametrize("nats", [9.0, 17.0, 20.0])
+def test_many_small_weights_beside_large_ones(ctx, dev, dtype, drafts, hd, nats):
+    """Eight keys, one in every 32 of the first two tiles, that weigh exp(nats) times as much as each of 100,000 others, and whose
+    values are 0: the result is what the others' weights add up to, 60 % to 0.003 % of all. As many sequences as the GPU has SMs hold
+    the same pages, so that a CTA has all keys of one and meets the large weights first.
+
+    A weight of f16 loses bits below 2^-14 of what it is rounded at. The kernel takes weights times 2^11 and the largest as 1 or
+    more, so what is lost is half a step of 2^-24, 2^-36 of the largest weight; against a sum of at least that weight it is
+    keys * 2^-36 of the largest value."""
+    import torch
+    n, sms = 100000, torch.cuda.get_device_properties(0).multi_processor_count
+    c = Case(ctx, dev, lens=[n + drafts], drafts=[drafts], hq=2, hkv=1, hd=hd, page=64, dtype=dtype, kv=dtype, mask="none", seed=141, scale=0.125)
+    c.q[:] = 8.0
+    c.k[:] = 0.0
+    c.v[:] = synth.round_to(1.0 + 0.25 * c.v, dtype)
+    large = c.cache_row(0, np.arange(8) * 32 + 5)
+    c.k[large, 0], c.v[large] = nats, 0.0
+    d = c.upload()
+    table = d["table"][:1].repeat(sms, 1).contiguous()
+    lens = torch.full((sms,), n + drafts, dtype=torch.int32, device="cuda")
+    starts = torch.arange(sms + 1, dtype=torch.int32, device="cuda") * drafts
+    q, mask, out = d["q"].repeat(sms, 1), d["mask"].repeat(sms, 1), d["out"].repeat(sms, 1)
+    pool = L.KvPool(ctx, page_rows=64, n_pages=c.n_pages, n_slots=sms, max_pages=c.max_pages, table=table, lens=lens, refs=d["refs"], stores=[d["k"], d["v"]],
+                    row_bytes=2 * hd)
+    ctx.tree_attn(pool, q, out, k_store=0, v_store=1, q_start=starts, n_seqs=sms, rows=sms * drafts, mask=mask, mask_words=c.words, n_q_heads=2, n_kv_heads=1,
+                  head_dim=hd, scale=c.scale, dtype=dtype, kv_dtype=dtype, workspace=d["work"], workspace_bytes=d["bytes"])
+    ctx.stream_sync()
+    pool.close()
+    rows = c.cache_row(0, np.arange(n))
+    want, size, terms = attention(c.q[:1, :hd], c.k[rows], c.v[rows], np.ones((1, n), bool), np.float32(c.scale))
+    tol = tolerance(want, size, terms, n, hd, dtype, True) + n * 2.0 ** -36 * np.abs(c.v).max()
+    err = np.abs(dev.get(out).reshape(-1, hd) - want)
+    assert (err <= tol).all(), f"{err.max():.3e} of {np.abs(want).max():.3e}"
