@@ -319,11 +319,14 @@ __device__ __forceinline__ size_t piece_at(size_t piece, unsigned head_dim, unsi
 
 // A block as the softmax groups need it, in shared memory; n == 0 ends the walk.
 struct __align__(16) TcUnit {
-    unsigned row0, len, block, kv_head;
+    unsigned row0, len, block_piece, kv_head;  // block * 4 + whole * 2 + piece: of 2^31 rows there are less than 2^25 blocks
     unsigned k0, n;         // key tiles k0 .. k0 + n
     unsigned drafted;       // drafted rows of the sequence
-    unsigned slot_piece;    // slot * 4 + whole * 2 + piece
+    unsigned slot;
     __device__ int ctx() const { return static_cast<int>(len - drafted); }
+    __device__ unsigned block() const { return block_piece >> 2; }
+    __device__ bool whole() const { return (block_piece & 2u) != 0; }
+    __device__ unsigned piece() const { return block_piece & 1u; }
 };
 
 // Infinities and NaNs in V rows of drafted rows were set to 0 for the product, because rows that do not
@@ -332,7 +335,7 @@ struct __align__(16) TcUnit {
 template <typename T, int HD>
 __device__ __noinline__ void add_bad_values(const TreeArgs& a, const TcUnit* unit, unsigned node, unsigned head, float m, float l, T* out, float* piece,
                                             unsigned c0, unsigned c1) {
-    const TreeSeq seq{unit->row0, unit->drafted, unit->ctx(), static_cast<int>(unit->len), unit->slot_piece >> 2};
+    const TreeSeq seq{unit->row0, unit->drafted, unit->ctx(), static_cast<int>(unit->len), unit->slot};
     const int first = max(seq.ctx, static_cast<int>(unit->k0) * kTcKeys), last = min(seq.len, static_cast<int>(unit->k0 + unit->n) * kTcKeys);
     const T* q = static_cast<const T*>(a.q) + static_cast<size_t>(seq.row0 + node) * a.q_stride + static_cast<size_t>(head) * HD;
     for (int pos = first; pos < last; pos++) {
@@ -387,7 +390,7 @@ __device__ __forceinline__ bool few_rows(const TreeArgs& a, const TcUnit* now, u
         met ^= 1u;
     };
     const unsigned n = now->n, qb = units & 1u, g = lane >> 2, c = lane & 3u, pair = warp & 3u;
-    const unsigned flat0 = now->block * a.block_rows, m_rows = rows_of(a, now->drafted, now->block);
+    const unsigned flat0 = now->block() * a.block_rows, m_rows = rows_of(a, now->drafted, now->block());
     const int len = static_cast<int>(now->len), ctx = now->ctx();
     const TreeSeq seq{now->row0, now->drafted, ctx, len, 0u};
     unsigned node[2];  // of rows g and g + 8
@@ -559,7 +562,7 @@ __device__ __forceinline__ bool few_rows(const TreeArgs& a, const TcUnit* now, u
     meet();
     const unsigned row = tid & 15u, c0 = (tid >> 4) * (HD / 16);
     if (row < m_rows) {
-        const bool whole = (now->slot_piece & 2u) != 0;
+        const bool whole = now->whole();
         float2 parts[4];
 #pragma unroll
         for (int x = 0; x < 4; x++) parts[x] = ml[x * 16 + row];
@@ -573,7 +576,7 @@ __device__ __forceinline__ bool few_rows(const TreeArgs& a, const TcUnit* now, u
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
         const unsigned flat = flat0 + row, node_r = flat / a.group, head = now->kv_head * a.group + flat % a.group;
         T* out = static_cast<T*>(a.out) + static_cast<size_t>(now->row0 + node_r) * a.out_stride + static_cast<size_t>(head) * HD;
-        const unsigned piece = blockIdx.x * 2 + (now->slot_piece & 1u);
+        const unsigned piece = blockIdx.x * 2 + now->piece();
         float* po = a.part_o + piece_at(piece, HD, 0, row);
         float y[HD / 16];
 #pragma unroll
@@ -793,7 +796,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         TcUnit* described = reinterpret_cast<TcUnit*>(tc_smem + S::kUnit);
         const auto publish = [&](unsigned n) {  // block `units`, to the softmax groups
             if (lane == 0) {
-                described[units % S::kUnits] = TcUnit{u.seq.row0, static_cast<unsigned>(u.seq.len), u.block, u.kv_head, u.k0, n, u.seq.n, u.seq.slot * 4 + (u.whole ? 2u : 0u) + u.piece};
+                described[units % S::kUnits] = TcUnit{u.seq.row0, static_cast<unsigned>(u.seq.len), u.block * 4 + (u.whole ? 2u : 0u) + u.piece, u.kv_head, u.k0, n, u.seq.n, u.seq.slot};
                 mbar_arrive(ufull + 8 * (units % S::kUnits));
             }
             __syncwarp();
@@ -929,8 +932,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const auto finish = [&] {
             const unsigned which = units - 1;  // the block's number
             const TcUnit* last = described + which % S::kUnits;
-            const bool whole = (last->slot_piece & 2u) != 0;
-            const unsigned flat0 = last->block * a.block_rows, m_rows = rows_of(a, last->drafted, last->block);
+            const bool whole = last->whole();
+            const unsigned flat0 = last->block() * a.block_rows, m_rows = rows_of(a, last->drafted, last->block());
             ok = __all_sync(0xffffffffu, ok && tc_wait(udone, (FEW ? big_units - 1 : which) & 1u, a.wait_limit, gave_up));
             tc_fence_after();
             ml[w * 128 + row] = make_float2(last_m, last_l);
@@ -946,7 +949,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if ((warp & 3u) * 32 < m_rows) {
                 const unsigned flat = flat0 + min(row, m_rows - 1), node = flat / a.group, head = last->kv_head * a.group + flat % a.group;
                 T* out = static_cast<T*>(a.out) + static_cast<size_t>(last->row0 + node) * a.out_stride + static_cast<size_t>(head) * HD;
-                float* po = a.part_o + piece_at(blockIdx.x * 2 + (last->slot_piece & 1u), HD, 0, row);
+                float* po = a.part_o + piece_at(blockIdx.x * 2 + last->piece(), HD, 0, row);
                 const unsigned c0 = w * (HD / 2);
 #pragma unroll 1
                 for (unsigned c = c0; c < c0 + HD / 2; c += 16) {
@@ -971,7 +974,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
                 if (row < m_rows) {
-                    if (!whole && w == 0) a.part_ml[(blockIdx.x * 2 + (last->slot_piece & 1u)) * kTcRows + row] = make_float2(top, total);
+                    if (!whole && w == 0) a.part_ml[(blockIdx.x * 2 + last->piece()) * kTcRows + row] = make_float2(top, total);
                     if (fix && total != 0.0f) add_bad_values<T, HD>(a, last, node, head, ref, total, out, whole ? nullptr : po, c0, c0 + HD / 2);
                 }
             }
@@ -1083,7 +1086,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const TcUnit* now = described + units % S::kUnits;
             const unsigned n = now->n;
             if (n == 0 && !pending) break;
-            const unsigned flat0 = now->block * a.block_rows, m_rows = rows_of(a, now->drafted, now->block);
+            const unsigned flat0 = now->block() * a.block_rows, m_rows = rows_of(a, now->drafted, now->block());
             if (FEW && n && m_rows <= kFewRows) {
                 if (pending) finish();
                 ok = few_rows<T, HD>(a, now, units, ring_t, met, ok);

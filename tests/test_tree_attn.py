@@ -831,3 +831,30 @@ def test_many_small_weights_beside_large_ones(ctx, dev, dtype, drafts, hd, nats)
     tol = tolerance(want, size, terms, n, hd, dtype, True) + n * 2.0 ** -36 * np.abs(c.v).max()
     err = np.abs(dev.get(out).reshape(-1, hd) - want)
     assert (err <= tol).all(), f"{err.max():.3e} of {np.abs(want).max():.3e}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drafts", [8, 30])
+def test_slots_past_two_to_the_thirty(ctx, dev, drafts):
+    """Infinities in a drafted V row are added by way of the page table: its row is that of the slot, not of another one that has the
+    same low bits."""
+    import torch
+    c = Case(ctx, dev, lens=[40, 40], drafts=[drafts, drafts], hq=2, hkv=1, hd=64, page=64, dtype=BF16, kv=BF16, mask=None, seed=151)
+    c.v[c.cache_row(0, np.array([40 - drafts]))[0], 5] = np.inf  # the first drafted row, which all see
+    want = c.run()
+    slots = 2 ** 30 + 4
+    table = torch.empty((slots, 1), dtype=torch.int32, device="cuda")
+    lens = torch.empty(slots, dtype=torch.int32, device="cuda")
+    for at, i in ((slots - 2, 0), (2, 1)):  # 2^30 + 2 and 2
+        table[at, 0], lens[at] = int(c.table[i, 0]), 40
+    d = c.d
+    pool = L.KvPool(ctx, page_rows=64, n_pages=c.n_pages, n_slots=slots, max_pages=1, table=table, lens=lens, refs=d["refs"], stores=[d["k"], d["v"]],
+                    row_bytes=128)
+    d["out"].fill_(c.fill)
+    ctx.tree_attn(pool, d["q"], d["out"], k_store=0, v_store=1, slots=dev.put(np.array([slots - 2, 2], np.int32)), q_start=d["starts"], n_seqs=2, rows=c.rows,
+                  n_q_heads=2, n_kv_heads=1, head_dim=64, scale=c.scale, dtype=BF16, kv_dtype=BF16, workspace=d["work"], workspace_bytes=d["bytes"])
+    ctx.stream_sync()
+    pool.close()
+    got = dev.get(d["out"])
+    assert (want[:drafts, 5::64] == np.inf).all() and np.isfinite(want[drafts:]).all()
+    assert np.array_equal(got, want)
