@@ -419,7 +419,8 @@ LOKAL_API int lokal_cuda_kv_pool_copy_pages(lokal_cuda_ctx* ctx, lokal_cuda_stre
  * order, move up behind the committed ones in every store, and the slot is cut behind them. accepted is
  * [n_seqs][max_accept], max_accept at most 256. A sequence with a bad list is left as it was. Rows move within the pages
  * that hold them, so drafted rows have to be the slot's own: fork a slot before its drafts are reserved or after they are
- * accepted, not between. */
+ * accepted, not between. A sequence with a row that would move into a page that another slot holds (refs above 1 before the
+ * call) counts as one with a bad list. */
 LOKAL_API int lokal_cuda_kv_pool_accept(lokal_cuda_ctx* ctx, lokal_cuda_stream s, lokal_kv_pool* pool, const uint32_t* slots,
                                         const int32_t* q_start, const int32_t* accepted, const int32_t* n_accepted, uint32_t max_accept,
                                         size_t n_seqs);

@@ -29,14 +29,15 @@ constexpr unsigned kPlanThreads = 1024;
 struct PoolWork {
     int* n_copies;   // copies in the list
     int* n_used;     // compact: used pages
+    int* seqs_done;  // accept: sequences that are done; 0 between calls
     int* copy_src;   // [n_pages] page
     int* copy_dst;   // [n_pages] page
     int* copy_rows;  // [n_pages] rows of the page that are copied
     int* free_list;  // [n_pages] the lowest free pages, ascending
     int* remap;      // [n_pages] compact: new page of a page that moves
     int* claim;      // [n_slots] first list entry that names the slot as its target
-    int* ent_new;    // [n_slots] per entry: its first place in free_list, -1 = skipped
-    int* ent_len;    // [n_slots] per entry: positions of the slot before the call (fork: of the source)
+    int* ent_new;    // [n_slots] per entry: its first place in free_list (accept: new length), -1 = skipped
+    int* ent_len;    // [n_slots] per entry: positions of the slot before the call (fork: of the source; accept: pages it holds)
     int* ent_cow;    // [n_slots] per entry: page that is copied before the slot writes to it, -1 = none
     int* arrived;    // [n_slots] accept: CTAs of a sequence that are done; 0 between calls
 };
@@ -45,6 +46,7 @@ __host__ __device__ inline PoolWork pool_work(int* w, unsigned n_pages, unsigned
     PoolWork p;
     p.n_copies = w;
     p.n_used = w + 1;
+    p.seqs_done = w + 2;
     w += 4;
     p.copy_src = w;
     p.copy_dst = p.copy_src + n_pages;
@@ -410,24 +412,21 @@ constexpr unsigned kMaxAccept = 256;
 // in place. The a_j ascend, so a_j >= j and a row is written only after every move that reads it: within a batch all
 // loads come before the first store, and a later source lies behind every target so far. The row numbers of the path
 // are worked out once per CTA.
+//
+// A row must not move into a page that another slot holds. Every CTA decides that, and the rest of what makes an entry
+// good, for itself and from the state before the call: table, lengths and counts are changed by the last CTA of the
+// launch, when all the others have read them. (Were a sequence cut as soon as it is done, a page that two sequences of the
+// list share would be shared for some CTAs of the other and not for the rest.)
 template <typename V>
 __global__ void __launch_bounds__(256) pool_accept_kernel(const PoolArgs a, const AcceptArgs t) {
     pdl_sync();
     __shared__ int from[kMaxAccept], to[kMaxAccept];
-    __shared__ int bad;
+    __shared__ int bad, held;
     const unsigned i = blockIdx.y;
     const unsigned slot = t.slots ? t.slots[i] : i;
     const PoolWork w = pool_work(a.work, a.n_pages, a.n_slots);
-    // A slot that an earlier sequence of the list names too is that sequence's, which may be cutting it meanwhile: the CTA
-    // leaves as a whole before it reads anything of the slot. (Were a part of its threads to see the length of before and a
-    // part that of after, some would go on with rows that nobody has worked out.)
-    bool taken = false;
-    for (unsigned k = threadIdx.x; k < i; k += 256) taken = taken || (t.slots ? t.slots[k] : k) == slot;
-    if (threadIdx.x == 0) bad = 0;
-    if (__syncthreads_or(taken)) {
-        if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.err_word, kErrPageRange);
-        return;
-    }
+    if (threadIdx.x == 0) bad = held = 0;
+    __syncthreads();
     const int drafts = t.q_start[i + 1] - t.q_start[i], count = t.counts[i];
     int len = 0, base = 0;
     bool ok = slot < a.n_slots && drafts >= 0 && count >= 0 && count <= drafts && count <= static_cast<int>(t.max_accept);
@@ -436,9 +435,9 @@ __global__ void __launch_bounds__(256) pool_accept_kernel(const PoolArgs a, cons
         base = len - drafts;
         ok = base >= 0 && len <= static_cast<int>(a.max_pages << a.page_shift);
     }
+    const int32_t* row = a.table + static_cast<size_t>(ok ? slot : 0) * a.max_pages;
     if (ok) {
         const int32_t* acc = t.accepted + static_cast<size_t>(i) * t.max_accept;
-        const int32_t* row = a.table + static_cast<size_t>(slot) * a.max_pages;
         for (int j = static_cast<int>(threadIdx.x); j < count; j += 256) {
             const int x = acc[j];
             if (x < 0 || x >= drafts || (j > 0 && acc[j - 1] >= x)) {
@@ -446,7 +445,7 @@ __global__ void __launch_bounds__(256) pool_accept_kernel(const PoolArgs a, cons
                 continue;
             }
             const int ps = row[(base + x) >> a.page_shift], pd = row[(base + j) >> a.page_shift];
-            if (!page_ok(a, ps) || !page_ok(a, pd)) {
+            if (!page_ok(a, ps) || !page_ok(a, pd) || (x != j && a.refs[pd] > 1)) {
                 bad = 1;
                 continue;
             }
@@ -454,16 +453,27 @@ __global__ void __launch_bounds__(256) pool_accept_kernel(const PoolArgs a, cons
             from[j] = (ps << a.page_shift) + ((base + x) & m);
             to[j] = (pd << a.page_shift) + ((base + j) & m);
         }
+        // a slot that an earlier sequence of the list names too is that sequence's
+        for (unsigned k = threadIdx.x; k < i; k += 256)
+            if ((t.slots ? t.slots[k] : k) == slot) bad = 1;
     }
     __syncthreads();
     ok = ok && !bad;
-    if (!ok) {
-        if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.err_word, kErrPageRange);
-        return;
+    const int want = base + count;
+    if (blockIdx.x == 0) {
+        // what the cut behind the path needs to know: the new length, and how far the slot's pages go
+        if (ok) {
+            int end = 0;
+            for (unsigned p = static_cast<unsigned>(pages_of(a, want)) + threadIdx.x; p < a.max_pages; p += 256)
+                if (row[p] >= 0) end = static_cast<int>(p) + 1;
+            if (end) atomicMax(&held, end);
+        } else if (threadIdx.x == 0) {
+            atomicOr(a.err_word, kErrPageRange);
+        }
     }
     const unsigned row_vecs = static_cast<unsigned>(a.row_bytes / sizeof(V));
     const unsigned long long vecs = static_cast<unsigned long long>(row_vecs) * a.n_stores;
-    for (unsigned long long e = static_cast<unsigned long long>(blockIdx.x) * 256 + threadIdx.x; e < vecs; e += gridDim.x * 256ull) {
+    for (unsigned long long e = static_cast<unsigned long long>(blockIdx.x) * 256 + threadIdx.x; ok && e < vecs; e += gridDim.x * 256ull) {
         V* base_v = static_cast<V*>(a.stores[e / row_vecs]) + e % row_vecs;
         constexpr int kBatch = 8;
         for (int j0 = 0; j0 < count; j0 += kBatch) {
@@ -476,20 +486,45 @@ __global__ void __launch_bounds__(256) pool_accept_kernel(const PoolArgs a, cons
                 if (j0 + j < count && from[j0 + j] != to[j0 + j]) base_v[static_cast<size_t>(to[j0 + j]) * row_vecs] = v[j];
         }
     }
-    // The cut behind the path: by the sequence's last CTA, when all have read the table (and in the one launch that the
-    // moves need; the count is back at 0 for the next call).
+    // The cuts behind the paths, by the launch's last CTA (in the one launch that the moves need; the counts are back at 0 for
+    // the next call).
     __syncthreads();
     if (threadIdx.x == 0) {
+        if (blockIdx.x == 0) {
+            w.ent_new[i] = ok ? want : -1;
+            w.ent_len[i] = held;
+        }
         __threadfence();
         bad = atomicAdd(w.arrived + i, 1) == static_cast<int>(gridDim.x) - 1;
+        if (bad) {
+            w.arrived[i] = 0;
+            __threadfence();
+            bad = atomicAdd(w.seqs_done, 1) == static_cast<int>(gridDim.y) - 1;
+            __threadfence();
+        }
     }
     __syncthreads();
     if (!bad) return;
-    if (threadIdx.x == 0) {
-        w.arrived[i] = 0;
-        a.lens[slot] = base + count;
+    if (threadIdx.x == 0) *w.seqs_done = 0;
+    unsigned lanes = 32;  // to a sequence: a few pages are behind its path
+    while (lanes > 1 && lanes * t.n_seqs > 256) lanes >>= 1;
+    for (unsigned k = threadIdx.x / lanes; k < t.n_seqs; k += 256 / lanes) {
+        const int cut = __ldcg(w.ent_new + k);
+        const unsigned end = static_cast<unsigned>(__ldcg(w.ent_len + k)), of = t.slots ? t.slots[k] : k;
+        if (cut < 0) continue;
+        if (threadIdx.x % lanes == 0) a.lens[of] = cut;
+        int32_t* pages = a.table + static_cast<size_t>(of) * a.max_pages;
+        for (unsigned p0 = static_cast<unsigned>(pages_of(a, cut)) + threadIdx.x % lanes; p0 < end; p0 += 4 * lanes) {
+            int old[4];
+#pragma unroll
+            for (unsigned j = 0; j < 4; j++) old[j] = p0 + j * lanes < end ? pages[p0 + j * lanes] : -1;
+#pragma unroll
+            for (unsigned j = 0; j < 4; j++) {
+                if (p0 + j * lanes < end) pages[p0 + j * lanes] = -1;
+                if (page_ok(a, old[j])) atomicSub(a.refs + old[j], 1);
+            }
+        }
     }
-    for (unsigned p = threadIdx.x; p < a.max_pages; p += 256) give_back(a, slot, p, base + count);
 }
 
 // ---- cache rows of token rows, the paged twin of kv_rows ----

@@ -343,3 +343,67 @@ def test_a_new_pool_is_ready_on_any_stream(ctx, dev):
         assert (store[:, 2 * page:2 * page + 5] == step).all() and (store[:, 2 * page + 5:] == -1).all()
         pool.close()
     ctx.stream_destroy(s)
+
+
+class CarefulModel(PoolModel):
+    """accept leaves a sequence as it was if a row would move into a page that another slot holds before the call."""
+
+    def accept(self, slots, n_rows, accepted, counts):
+        refs, seen, counts = self.refs.copy(), set(), list(counts)
+        for i, (s, n) in enumerate(zip(slots, n_rows)):
+            if s in seen or s >= self.n_slots:
+                continue
+            seen.add(s)
+            base = int(self.lens[s]) - n
+            moves = [base + j for j, a in enumerate(list(accepted[i])[:max(0, counts[i])]) if a != j and 0 <= base + j < self.max_pages * self.page]
+            if any(refs[self.table[s, p // self.page]] > 1 for p in moves if self.table[s, p // self.page] >= 0):
+                counts[i] = -1
+        super().accept(slots, n_rows, accepted, counts)
+
+
+@pytest.mark.gpu
+def test_accept_does_not_move_rows_into_a_page_that_another_slot_holds(ctx, dev):
+    r = Rig(ctx, dev, 8, 40, 6, 8, 3, 40, 29)
+    r.m.__class__ = CarefulModel
+    r.both("reserve", [0], [8 + 16])  # 8 committed rows, two pages of drafted ones
+    r.both("fork", [0, 0], [1, 2])
+    r.same("forked between drafting and accepting")
+    r.accept([0], [16], [[1, 2]], [2])
+    assert r.m.bad and r.m.lens[0] == 24
+    r.same("shared target")
+    r.accept([0, 1], [16, 16], [[0, 1], [0, 9]], [2, 2])  # no row of 0 moves, so it is cut; one of 1 does, and would into a shared page
+    assert r.m.bad and r.m.lens[0] == 10 and r.m.lens[1] == 24
+    r.same("only what moves counts")
+    r.accept([1, 2], [16, 16], [[0, 0], [5, 8]], [0, 2])  # 1 gives its pages back in the call in which 2 would write into one of them
+    assert r.m.bad and r.m.lens[1] == 8 and r.m.lens[2] == 24
+    r.same("the counts are those of before the call")
+    r.accept([2], [8], [[3, 7]], [2])  # the last page is its own by now
+    assert not r.m.bad and r.m.lens[2] == 18
+    r.same("its own page")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page,n_slots,n_stores,width", [(8, 12, 40, 512), (16, 70, 3, 24), (16, 300, 2, 8)])
+def test_accept_on_slots_that_share_pages_in_any_order(ctx, dev, page, n_slots, n_stores, width):
+    r = Rig(ctx, dev, page, 40 * n_slots // 8, n_slots, 10, n_stores, width, 31)
+    r.m.__class__ = CarefulModel
+    rng = np.random.default_rng(31)
+    refused = 0
+    for step in range(12):
+        roots = n_slots // 4
+        r.both("truncate", np.arange(n_slots), None)
+        r.both("reserve", np.arange(roots), rng.integers(page, 5 * page, roots))
+        r.both("fork", rng.integers(0, roots, n_slots - roots), np.arange(roots, n_slots))
+        some = rng.permutation(n_slots)[:n_slots // 3]
+        r.both("reserve", some, np.minimum(10 * page, r.m.lens[some] + rng.integers(1, 2 * page, len(some))))
+        r.same(f"step {step}: made")
+        slots = rng.permutation(n_slots)
+        n = np.array([int(rng.integers(0, r.m.lens[s] + 1)) for s in slots])
+        counts = np.array([int(rng.integers(0, min(x, 12) + 1)) for x in n])
+        acc = np.zeros((n_slots, 12), np.int64)
+        for i in range(n_slots):
+            acc[i, :counts[i]] = np.arange(counts[i]) if rng.random() < 0.3 else np.sort(rng.permutation(n[i])[:counts[i]])
+        r.accept(slots, n, acc, counts)
+        refused += r.m.bad
+        r.same(f"step {step}: accepted")
+    assert refused
