@@ -376,7 +376,8 @@ LOKAL_API int lokal_cuda_kv_stage(lokal_cuda_ctx* ctx, lokal_cuda_stream s, cons
  * issue them in one order (one stream, or streams ordered by events). Results depend only on the state and the lists:
  * new pages are the lowest-numbered free ones, in list order. An entry that cannot be carried out (a slot out of range
  * or named by an earlier entry, a length the table cannot hold, no free page) is left undone, the others are not, and
- * the next lokal_cuda_stream_sync returns LOKAL_ERR_PAGE_RANGE or LOKAL_ERR_NO_PAGES.
+ * the next lokal_cuda_stream_sync returns LOKAL_ERR_PAGE_RANGE or LOKAL_ERR_NO_PAGES (the latter if there was any of it, as
+ * the rest of a step then finds rows missing).
  *
  * page_rows: a power of two, 8 to 256. n_pages * page_rows at most 2^31 - 1, max_pages * page_rows at most 2^31 - 256. row_bytes even;
  * with stores and row_bytes multiples of 16 bytes, copies use 16-byte accesses. A list has at most n_slots entries

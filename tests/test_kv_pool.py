@@ -407,3 +407,18 @@ def test_accept_on_slots_that_share_pages_in_any_order(ctx, dev, page, n_slots, 
         refused += r.m.bad
         r.same(f"step {step}: accepted")
     assert refused
+
+
+@pytest.mark.gpu
+def test_a_step_that_runs_out_of_pages_says_so(ctx, dev):
+    """What follows in the step finds the rows missing too; the status is the one that a scheduler acts on."""
+    import torch
+    r = Rig(ctx, dev, 8, 4, 3, 4, 2, 8, 37)
+    out = torch.zeros(24, dtype=torch.int32, device="cuda")
+    r.both("reserve", [0, 1], [16, 24])
+    r.pool.rows(out, rows=24, slot0=1)
+    ctx.tree_plan(r.pool, slots=r.ints([1]), q_start=r.ints([0, 24]), n_seqs=1, rows=24, cache_rows=out)
+    assert r.m.no_pages
+    r.same("reserve, rows and plan of a step")
+    r.pool.rows(out, rows=24, slot0=1)
+    assert r.sync() == capi.ERR_POS_RANGE
