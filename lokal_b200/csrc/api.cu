@@ -12,6 +12,22 @@
 
 using lokal::DeviceGuard;
 
+namespace lokal {
+
+// The first that holds: what the others may follow from comes first.
+int fail_of_bits(lokal_cuda_ctx* ctx, unsigned bits) {
+    if (bits & kErrTimeout) return ctx->fail(LOKAL_ERR_TIMEOUT, "a device-side wait on a staged copy gave up");
+    // ahead of what follows from it in the same step: rows of positions that were not granted
+    if (bits & kErrNoPages) return ctx->fail(LOKAL_ERR_NO_PAGES, "the cache pool has too few free pages (the entries that did not fit were left as they were)");
+    if (bits & kErrPosRange)
+        return ctx->fail(LOKAL_ERR_POS_RANGE, "a position was negative or beyond the KV cache (its row was not stored)");
+    if (bits & kErrPageRange)
+        return ctx->fail(LOKAL_ERR_PAGE_RANGE, "a slot, page, length or drafted row of a cache pool call was out of range or named twice (its entry was skipped)");
+    return ctx->fail(LOKAL_ERR_ID_RANGE, "a token id was out of range for the table (its row was zero-filled)");
+}
+
+}  // namespace lokal
+
 namespace {
 
 constexpr const char* kVersion = "lokal_cuda 0.1 (sm_100a)";
@@ -136,14 +152,7 @@ int read_error_word(lokal_cuda_ctx* ctx, cudaStream_t s) {
     if (bits == 0) return LOKAL_OK;
     LOKAL_CUDA_TRY(ctx, cudaMemsetAsync(ctx->err_word, 0, sizeof(unsigned), s));
     LOKAL_CUDA_TRY(ctx, cudaStreamSynchronize(s));
-    if (bits & lokal::kErrTimeout) return ctx->fail(LOKAL_ERR_TIMEOUT, "a device-side wait on a staged copy gave up");
-    // ahead of what follows from it in the same step: rows of positions that were not granted
-    if (bits & lokal::kErrNoPages) return ctx->fail(LOKAL_ERR_NO_PAGES, "the cache pool has too few free pages (the entries that did not fit were left as they were)");
-    if (bits & lokal::kErrPosRange)
-        return ctx->fail(LOKAL_ERR_POS_RANGE, "a position was negative or beyond the KV cache (its row was not stored)");
-    if (bits & lokal::kErrPageRange)
-        return ctx->fail(LOKAL_ERR_PAGE_RANGE, "a slot, page, length or drafted row of a cache pool call was out of range or named twice (its entry was skipped)");
-    return ctx->fail(LOKAL_ERR_ID_RANGE, "a token id was out of range for the table (its row was zero-filled)");
+    return lokal::fail_of_bits(ctx, bits);
 }
 
 }  // namespace

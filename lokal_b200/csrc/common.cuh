@@ -28,7 +28,7 @@ namespace lokal {
 
 constexpr int kSmCountB200 = 148;
 
-// Device-side error word bits (read back by lokal_cuda_stream_sync).
+// Device-side error word bits (read back by lokal_cuda_stream_sync and lokal_cuda_pass_run_host).
 enum : unsigned { kErrIdRange = 1u, kErrTimeout = 2u, kErrPosRange = 4u, kErrNoPages = 8u, kErrPageRange = 16u };
 
 }  // namespace lokal
@@ -70,6 +70,11 @@ struct lokal_cuda_ctx {
         return code;
     }
 };
+
+namespace lokal {
+// The status that the bits of the error word stand for (api.cu).
+int fail_of_bits(lokal_cuda_ctx* ctx, unsigned bits);
+}  // namespace lokal
 
 struct lokal_cuda_graph {
     cudaGraph_t graph = nullptr;

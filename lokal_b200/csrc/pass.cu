@@ -355,14 +355,12 @@ int lokal_cuda_pass_run_host(lokal_cuda_ctx* ctx, lokal_cuda_pass* P, const loka
     LOKAL_CUDA_TRY(ctx, cudaMemcpyAsync(out_host, P->out_dev, rows * c.hidden * P->es, cudaMemcpyDeviceToHost, ks));
     LOKAL_CUDA_TRY(ctx, cudaStreamSynchronize(ks));
     LOKAL_CUDA_TRY(ctx, cudaStreamSynchronize(cs));
-    // device-side error word (out-of-range ids, bounded waits)
+    // device-side error word
     LOKAL_CUDA_TRY(ctx, cudaMemcpy(ctx->err_word_host, ctx->err_word, sizeof(unsigned), cudaMemcpyDeviceToHost));
     const unsigned bits = *ctx->err_word_host;
     if (bits) {
         LOKAL_CUDA_TRY(ctx, cudaMemset(ctx->err_word, 0, sizeof(unsigned)));
-        if (bits & lokal::kErrTimeout) return ctx->fail(LOKAL_ERR_TIMEOUT, "a device-side wait on a staged copy gave up");
-        if (bits & lokal::kErrPosRange) return ctx->fail(LOKAL_ERR_POS_RANGE, "a position was negative or beyond the KV cache (its row was not stored)");
-        return ctx->fail(LOKAL_ERR_ID_RANGE, "a token id was out of range for the table (its row was zero-filled)");
+        return lokal::fail_of_bits(ctx, bits);
     }
     return LOKAL_OK;
 }

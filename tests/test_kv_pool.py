@@ -422,3 +422,24 @@ def test_a_step_that_runs_out_of_pages_says_so(ctx, dev):
     r.same("reserve, rows and plan of a step")
     r.pool.rows(out, rows=24, slot0=1)
     assert r.sync() == capi.ERR_POS_RANGE
+
+
+@pytest.mark.gpu
+def test_a_host_pass_reports_what_a_pool_call_before_it_met(ctx, dev):
+    """run_host returns with the errors of the context, whichever call met them."""
+    import torch
+    from synth import BF16
+    from test_gpu_pass import build_pass, inputs_on, make_case, pass_inputs
+    cfg, a = make_case(BF16)
+    p = build_pass(ctx, dev, cfg, a, slots=2)
+    th = inputs_on("host", dev, cfg, a)
+    out = torch.zeros(cfg.rows, cfg.hidden, dtype=dev.tdt[BF16]).pin_memory()
+    r = Rig(ctx, dev, 8, 4, 3, 4, 2, 8, 39)
+    for slots, lens, status in [([0], [33], capi.ERR_PAGE_RANGE), ([0, 1], [16, 24], capi.ERR_NO_PAGES)]:
+        r.pool.reserve(r.ints(slots), r.ints(lens), n=len(slots))
+        torch.cuda.synchronize()
+        with pytest.raises(L.LokalCudaError) as e:
+            p.run_host(pass_inputs(cfg, th, 7), out)
+        assert e.value.status == status
+        p.run_host(pass_inputs(cfg, th, 7), out)
+    p.close()
