@@ -10,6 +10,7 @@ computes on the CPU.
 from __future__ import annotations
 
 import ctypes as C
+import weakref
 
 import numpy as np
 
@@ -52,10 +53,13 @@ class Context:
             raise LokalCudaError(rc, f"lokal_cuda_create(device={device}) failed")
         self._h = h
         self.device = device
+        self._pools = weakref.WeakSet()  # go before the context
 
     # -- plumbing ---------------------------------------------------------
     def close(self):
         if getattr(self, "_h", None):
+            for pool in list(self._pools):
+                pool.close()
             self._lib.lokal_cuda_destroy(self._h)
             self._h = None
 
@@ -338,6 +342,7 @@ class KvPool:
         ctx._check(self._lib.lokal_cuda_kv_pool_create(ctx._h, page_rows, n_pages, n_slots, max_pages, _ptr(table), _ptr(lens), _ptr(refs),
                                                        addrs, len(stores), row_bytes, C.byref(h)))
         self._h = h
+        ctx._pools.add(self)
 
     @property
     def handle(self):

@@ -443,3 +443,36 @@ def test_a_host_pass_reports_what_a_pool_call_before_it_met(ctx, dev):
         assert e.value.status == status
         p.run_host(pass_inputs(cfg, th, 7), out)
     p.close()
+
+
+class FakeLib:
+    """Stands in for the library: hands out a handle and remembers what is destroyed."""
+
+    def __init__(self):
+        self.gone = []
+
+    def lokal_cuda_create(self, device, out):
+        out._obj.value = 7
+        return capi.OK
+
+    def lokal_cuda_kv_pool_create(self, *args):
+        args[-1]._obj.value = 0x1234
+        return capi.OK
+
+    def lokal_cuda_kv_pool_destroy(self, ctx, pool):
+        self.gone.append(("pool", ctx.value, pool.value))
+        return capi.OK
+
+    def lokal_cuda_destroy(self, ctx):
+        self.gone.append(("context", ctx.value))
+
+
+def test_a_context_that_is_closed_first_takes_its_pools_along(monkeypatch):
+    monkeypatch.setattr(capi, "load", FakeLib)
+    ctx = L.Context(0)
+    made = [L.KvPool(ctx, page_rows=16, n_pages=1, n_slots=1, max_pages=1, table=1, lens=1, refs=1, stores=[1], row_bytes=16) for _ in range(2)]
+    made[0].close()
+    ctx.close()
+    made[1].close()
+    ctx.close()
+    assert ctx._lib.gone == [("pool", 7, 0x1234), ("pool", 7, 0x1234), ("context", 7)]
