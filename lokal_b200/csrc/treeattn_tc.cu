@@ -24,7 +24,8 @@
 // sequence: 46 us before, 54), larger blocks in the same call run 6 % slower, and with head size 128, where a tile's copy takes
 // twice the time, it won 3 % at best and lost 25 % at short lengths, so those keep to the other way.
 // An accumulator is rescaled only when the maximum has grown by more than 2^lag since it was last set, so that most tiles
-// leave it alone. Weights are rounded to the cache's type for the product (half a step each, as the values they multiply
+// leave it alone. A row's reference moves by its own scores only: the warp's other rows may be another sequence's, or what an
+// earlier call left in the tile. Weights are rounded to the cache's type for the product (half a step each, as the values they multiply
 // were); sums, maxima and scores are f32. bf16 has the exponents of f32 and takes weights of up to 2^8 and down to 2^-126. f16
 // loses bits below 2^-14, so there weights are taken times 2^11 with a lag of 2^4 (at most 2^15): half a step each down to
 // 2^-25 of the largest, and 2^-36 of it below that, where 100,000 keys of 2^-25 are 0.3 % of a row. Sums and accumulators
@@ -468,7 +469,7 @@ __device__ __forceinline__ bool few_rows(const TreeArgs& a, const TcUnit* now, u
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const float before = mx[h];
-                mx[h] = fmaxf(before, top[h]);
+                if (top[h] > before + Weights<T>::kLag) mx[h] = top[h];
                 f[h] = before == -INFINITY ? 0.0f : ex2(before - mx[h]);
                 sum[h] *= f[h];
             }
@@ -1015,7 +1016,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (top != -INFINITY) top *= scale;
             if (__any_sync(0xffffffffu, top > m + Weights<T>::kLag)) {
                 const float before = m;
-                m = fmaxf(m, top);
+                if (top > m + Weights<T>::kLag) m = top;
                 const float f = before == -INFINITY ? 0.0f : ex2(before - m);
                 l *= f;
                 if (begun) {

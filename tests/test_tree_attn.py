@@ -858,3 +858,32 @@ def test_slots_past_two_to_the_thirty(ctx, dev, drafts):
     got = dev.get(d["out"])
     assert (want[:drafts, 5::64] == np.inf).all() and np.isfinite(want[drafts:]).all()
     assert np.array_equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hq,hkv,hd,drafts", [(14, 2, 128, 40), (14, 2, 64, 40), (100, 1, 128, 3), (100, 1, 64, 3), (2, 1, 64, 2)])
+def test_rows_of_a_tile_that_are_nobodys_change_no_bit(ctx, dev, dtype, hq, hkv, hd, drafts):
+    """A tile of 128 query rows holds as many as divide by the query heads to a key head. What lies in the rest is what an earlier
+    call left there, here one with large scores. Nor do the rows of other sequences that share a tile matter."""
+    n = 160
+    c = Case(ctx, dev, lens=np.full(n, 700), drafts=np.full(n, drafts), hq=hq, hkv=hkv, hd=hd, dtype=dtype, kv=dtype, mask=None, seed=161)
+    other = Case(ctx, dev, lens=np.full(n, 300), drafts=np.full(n, drafts), hq=hq // hkv, hkv=1, hd=hd, dtype=dtype, kv=dtype, mask=None, seed=162)
+    other.q *= 64.0
+    big = Case(ctx, dev, lens=np.full(n, 300), drafts=np.full(n, 128), hq=1, hkv=1, hd=hd, dtype=dtype, kv=dtype, mask=None, seed=163)
+    big.q *= 64.0
+    first = c.run()
+    other.upload()
+    big.upload()
+    for _ in range(5):
+        other.call()
+        big.call()
+        c.call()
+        ctx.stream_sync()
+        assert np.array_equal(dev.get(c.d["out"]), first)
+    # every second sequence's rows with scores 64 times as large: the others' results stay
+    c.d["q"].view(n, drafts, -1)[::2] *= 64.0
+    c.call()
+    ctx.stream_sync()
+    again = dev.get(c.d["out"]).reshape(n, -1)
+    assert np.array_equal(again[1::2], first.reshape(n, -1)[1::2])
