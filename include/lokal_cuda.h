@@ -368,8 +368,9 @@ LOKAL_API int lokal_cuda_kv_stage(lokal_cuda_ctx* ctx, lokal_cuda_stream s, cons
  *   lens  [n_slots]             positions the slot holds
  *   refs  [n_pages]             table entries that name the page; 0 = free
  * lokal_cuda_kv_pool_reset makes them those of an empty pool; a program may also fill them itself, or save and restore
- * them, as long as every slot has the pages of its lens positions and refs counts them. (A linear cache is the table
- * [slot][i] = slot * max_pages + i with every refs 1.)
+ * them, as long as every slot has the pages of its lens positions, -1 behind them, and refs counts the entries. (A linear
+ * cache is the table [slot][i] = slot * max_pages + i with every refs 1 and lens that the program sets. Its pages behind lens
+ * are what the calls that grow and cut slots do not expect: it takes rows, copy_pages, tree_plan and tree_attn.)
  *
  * Lists (slots, lengths, pages) are device arrays: a decode loop can run these calls with no host round trip and inside
  * a captured graph; no call allocates. The calls on one pool read and rewrite its state and share its scratch memory:
@@ -456,7 +457,11 @@ LOKAL_API size_t lokal_cuda_tree_attn_workspace(const lokal_cuda_ctx* ctx, size_
  * k_store, v_store: numbers of the pool's stores; their rows start with n_kv_heads * head_dim elements of kv_dtype.
  * q, out: [rows][n_q_heads * head_dim] of dtype at the given row strides (elements); out must not overlap q.
  * Types F32 / F16 / BF16, any of them for either; scores, maxima and sums are f32. Where q and the cache have the same
- * 16-bit type, the weights are rounded to it for their product with V; every other pair has the accuracy of f32 products.
+ * 16-bit type, the weights are rounded to it for their product with V (half a step each; of f16, those below 2^-25 of the
+ * row's largest by up to 2^-36 of that); every other pair has the accuracy of f32 products. An infinity in a K row that a row
+ * sees makes the key's score infinite: with -inf the key weighs nothing, with +inf the row is NaN. One in a V row is the result
+ * of its column; with a weight of 0 it may be NaN there, or nothing. A row's result depends, bit for bit, on its own sequence
+ * and on how the keys of the call are dealt to the GPU's SMs, which the call's shapes and lengths decide.
  * head_dim up to 256.
  * workspace: device memory, 16-byte aligned, of lokal_cuda_tree_attn_workspace bytes, used until the call is done: calls
  * that may overlap need one each. Nothing of it has to be kept or cleared between calls. */

@@ -13,8 +13,9 @@
 // handed out in list order (prefix sums, never the order in which atomics arrive; the atomics on refs are integer
 // adds, which commute). An entry that cannot be carried out is skipped and reported at the next synchronisation.
 //
-// Bound by memory: the integers are a few kilobytes, the rows are what costs. A call is two launches, a plan by one
-// CTA and an apply over the whole GPU, joined by programmatic dependent launch.
+// Bound by memory: the integers are a few kilobytes, the rows are what costs. Calls that hand out pages (reserve, fork) and
+// compact are two launches, a plan by one CTA and an apply over the whole GPU, joined by programmatic dependent launch; the
+// others are one.
 #include "common.cuh"
 #include "kvpool.cuh"
 

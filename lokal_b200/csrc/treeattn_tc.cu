@@ -20,9 +20,9 @@
 // warps whose lanes hold the rows compute 128 keys by 32 rows in turn. With head size 64, and where sequences have few rows on
 // average, such blocks are taken by the softmax warps themselves: products of 16 rows by 32 keys a warp, from the same ring,
 // every key's weight in a thread of its own (few_rows). Single tokens of 256 sequences of up to 4,096 keys, 32 heads over 4:
-// 181 us before, 148 so; 8 of 131,072 keys: 212 and 183 (5.9 TB/s). What it costs: blocks end slower (one key tile to a
-// sequence: 46 us before, 54), larger blocks in the same call run 6 % slower, and with head size 128, where a tile's copy takes
-// twice the time, it won 3 % at best and lost 25 % at short lengths, so those keep to the other way.
+// 171 us without it, 144 with it; 8 of 131,072 keys: 206 and 185 (5.8 TB/s). What it costs: blocks end slower (one key tile to
+// a sequence: 46 us without it, 50 to 52 with it), larger blocks in the same call run 6 % slower, and with head size 128, where a
+// tile's copy takes twice the time, it won 3 % at best and lost 25 % at short lengths, so those keep to the other way.
 // An accumulator is rescaled only when the maximum has grown by more than 2^lag since it was last set, so that most tiles
 // leave it alone. A row's reference moves by its own scores only: the warp's other rows may be another sequence's, or what an
 // earlier call left in the tile. Weights are rounded to the cache's type for the product (half a step each, as the values they multiply
